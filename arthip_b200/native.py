@@ -64,6 +64,15 @@ SIGNATURES: dict[str, tuple] = {
     "ah_conv3x3_destroy": (None, [_vp]),
     "ah_conv3x3_run_noalloc": (_i32, [_i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp,
                                       _cp, _i32]),
+    "ah_norm_create": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(_vp), _cp, _i32]),
+    "ah_norm_run": (_i32, [_vp, _vp, _vp, _cp, _i32]),
+    "ah_norm_destroy": (None, [_vp]),
+    "ah_rope_create": (_i32, [_i32, _vp, ctypes.POINTER(_vp), _cp, _i32]),
+    "ah_rope_run": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _cp, _i32]),
+    "ah_rope_destroy": (None, [_vp]),
+    "ah_attn_create": (_i32, [_i32, _vp, _i32, _vp, _vp, _vp, _vp, ctypes.POINTER(_vp), _cp, _i32]),
+    "ah_attn_run": (_i32, [_vp, _vp, _vp, _cp, _i32]),
+    "ah_attn_destroy": (None, [_vp]),
     "ah_test_set_conv_fault_hook": (None, [_i32, _i32]),
     "ah_convert_float_to_float16": (_i32, [_vp, _sz, _i32, _cp, _i32, _i32, _vp, _sz, _szp, _cp, _i32]),
     "ah_load_onnx": (_i32, [_vp, _sz, _cp, _i64, _i64, _vp, _sz, _szp, _cp, _i32]),

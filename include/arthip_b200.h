@@ -202,6 +202,138 @@ int ah_conv3x3_run_noalloc(int device, int C, int M, const uint16_t* w_oihw_f16,
                            const void* in_nhwc, int H, int W, const void* add1, const void* add2,
                            void* out_nhwc, void* stream, char* err, int errlen);
 
+/* ------------------------------------------------------------------------------
+ * Token operators on device tensors (no counterpart in the reference; additions of this
+ * library), for the layers that stand between conv layers in attention-based restoration
+ * models. A token is a pixel or patch of a frame; rows are tokens, so a conv layer's NHWC
+ * frame is [tokens][channels] as it stands. Element types: 0 = fp16, 1 = bf16. Sums,
+ * statistics and softmax weights' sums are fp32.
+ *
+ * A handle holds uploaded parameters only and does not change after creation: runs of one
+ * handle may overlap on any streams and threads and be captured into CUDA graphs. A run is
+ * asynchronous on `stream` (cudaStream_t of the handle's device, NULL = legacy default),
+ * allocates nothing and leaves the caller's current device as it was. Strides count
+ * elements; 0 means packed. Inputs may be slices of one buffer. Return codes as above; a run
+ * that returns 1 has launched nothing. Destroy a handle only when its runs have finished.
+ * ---------------------------------------------------------------------------- */
+
+/* The norms before and after a block with its gate and residual scale, in one pass:
+ *   out  = x + residual_scale * layer_scale[c] * act(gate) * post(y)
+ *   norm = pre(out), then * (1 + mod_scale) + mod_shift
+ * post and pre: 0 none, 1 RMS norm v / sqrt(mean(v^2) + eps), 2 layer norm
+ * (v - mean) / sqrt(var + eps); then * weight[c] (+ bias[c]). gate_act: 0 the gate as it is,
+ * 1 sigmoid, 2 tanh, 3 SiLU. The pre-norm reads the sum before it is rounded to `out`. */
+typedef struct {
+  int dtype;
+  int channels; /* 1..8192 */
+  int post_norm, pre_norm;
+  float post_eps, pre_eps;
+  int gate_act;
+  float residual_scale;
+} ah_norm_desc;
+/* x [rows][channels]; y, or NULL for a pre-norm of x alone (then out and gate are NULL too);
+ * gate [rows / rows_per_gate][channels] or NULL; mod_scale and mod_shift
+ * [rows / rows_per_mod][channels], each or both NULL, with one stride; out and norm, at least
+ * one of them. Row r uses gate row r / rows_per_gate. A row that all rows share has
+ * rows_per_gate >= rows. An output may be x or y itself (same pointer and stride), or overlap
+ * no input. */
+typedef struct {
+  int64_t rows;
+  const void* x;
+  const void* y;
+  const void* gate;
+  const void* mod_scale;
+  const void* mod_shift;
+  void* out;
+  void* norm;
+  int64_t x_stride, y_stride, gate_stride, mod_stride, out_stride, norm_stride;
+  int64_t rows_per_gate, rows_per_mod;
+} ah_norm_io;
+typedef struct ah_norm ah_norm;
+/* Weights are host arrays of `channels` floats, or NULL for ones (biases: zeros). */
+int ah_norm_create(int device, const ah_norm_desc* desc, const float* post_weight, const float* post_bias,
+                   const float* pre_weight, const float* pre_bias, const float* layer_scale, ah_norm** out, char* err,
+                   int errlen);
+int ah_norm_run(ah_norm* h, const ah_norm_io* io, void* stream, char* err, int errlen);
+void ah_norm_destroy(ah_norm* h);
+
+/* Rotary positions over 1 to 3 axes (time, height, width): pairs of a head's elements turn by
+ * position * frequency, (a, b) -> (a cos - b sin, a sin + b cos). axis_dims[i] (even)
+ * elements belong to axis i, one axis after another from element 0; elements behind them are
+ * copied. Frequencies of axis i: theta[i]^(-2j / axis_dims[i]), j = 0 .. axis_dims[i] / 2 - 1.
+ * layout 0: pair j of an axis is elements j and j + axis_dims[i] / 2 of its section;
+ * layout 1: elements 2j and 2j + 1 of its section;
+ * layout 2: one spectrum over the whole rotated part of R elements: pair p is elements p and
+ *   p + R / 2 with frequency theta^(-2p / R), and belongs to the axis whose section of pairs
+ *   (axis_dims[i] / 2 each, one after another) holds p.
+ * inverse: turns the other way. */
+typedef struct {
+  int dtype;
+  int head_dim; /* 2..512 */
+  int axes;
+  int axis_dims[3];
+  double theta[3];
+  int layout;
+  int inverse;
+} ah_rope_desc;
+/* [tokens][heads][head_dim] by its strides; out may be in itself (same strides). */
+typedef struct {
+  const void* in;
+  void* out;
+  int heads; /* 1..1024 */
+  int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride;
+} ah_rope_io;
+typedef struct ah_rope ah_rope;
+int ah_rope_create(int device, const ah_rope_desc* desc, ah_rope** out, char* err, int errlen);
+/* positions: device fp32 [axes][tokens], whole or fractional. q and k turn in one launch;
+ * either may be NULL. */
+int ah_rope_run(ah_rope* h, int64_t tokens, const float* positions, const ah_rope_io* q, const ah_rope_io* k,
+                void* stream, char* err, int errlen);
+void ah_rope_destroy(ah_rope* h);
+
+/* Attention, out = softmax(scores) v, over documents (frames, windows, clips) packed one after
+ * another. For query i and key j of one document:
+ *   s = scale * (q . k);  s = cap * tanh(s / cap) when cap > 0;
+ *   s -= sum over axes of slopes[head][axis] * |q_position - k_position|
+ * mask 0: every key of the document. mask 1 (causal): keys j <= i + (keys - queries), counted
+ * in the document, and the document's first prefix keys. A query that sees no key gets zeros.
+ * Query head h reads key head h / (q_heads / kv_heads). */
+typedef struct {
+  int dtype;
+  int q_heads, kv_heads;
+  int head_dim; /* a multiple of 8, up to 128 */
+  float scale;  /* > 0 */
+  float cap;    /* 0 = none */
+  int mask;
+  int axes;     /* of the distance bias, 0..3 */
+} ah_attn_desc;
+/* q, out [q_offsets[docs]][q_heads][head_dim]; k, v [k_offsets[docs]][kv_heads][head_dim], by
+ * strides that are multiples of 8 elements, from 16-byte aligned pointers; out overlaps no
+ * input. positions: device fp32 [axes][total queries or keys]. k_lens: device int32 [docs],
+ * the keys in use of each document (from its first; clamped to its capacity), or NULL for all:
+ * it is read on the device, so that a captured run follows a cache as it grows. Memory behind
+ * the keys in use may hold anything; a NaN or infinity among a document's values in use may
+ * reach any query of that document. Tokens outside every document are not touched. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+  const float* q_positions;
+  const float* k_positions;
+  const int* k_lens;
+} ah_attn_io;
+typedef struct ah_attn ah_attn;
+/* Host arrays: q_offsets and k_offsets of docs + 1 token offsets from 0 (documents may be
+ * empty); prefix of docs lengths, or NULL; slopes [q_heads][axes], or NULL without axes. */
+int ah_attn_create(int device, const ah_attn_desc* desc, int docs, const int64_t* q_offsets,
+                   const int64_t* k_offsets, const int64_t* prefix, const float* slopes, ah_attn** out, char* err,
+                   int errlen);
+int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int errlen);
+void ah_attn_destroy(ah_attn* h);
+
 /* Test-only failure-path hook (no counterpart in the reference). For tensor-core conv launches made after the call, in this process:
  * every pipeline wait is bounded by wait_limit_ms (1..4000) instead of 4 s, and every CTA
  * arms the slot of its input row `stall_row` (counted from the CTA's first row) without
