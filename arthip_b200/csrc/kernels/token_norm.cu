@@ -14,6 +14,7 @@
 #include "tokens.h"
 
 #include <algorithm>
+#include <atomic>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,18 +23,25 @@ namespace ah {
 
 namespace {
 
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ void from_f(float v, __half* o) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f2(float a, float b, __half2* o) { *o = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void from_f2(float a, float b, __nv_bfloat162* o) { *o = __floats2bfloat162_rn(a, b); }
+
 template <typename T>
-__device__ __forceinline__ float to_f(T v);
+struct Two;
 template <>
-__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+struct Two<__half> {
+  using type = __half2;
+};
 template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
 
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
@@ -41,18 +49,56 @@ struct alignas(V * sizeof(T)) Vec {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-  const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ __forceinline__ Vec<T, V> load(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& u, float (&f)[V]) {
+  if constexpr (V % 2 == 0) {
+    const auto* p = reinterpret_cast<const typename Two<T>::type*>(&u);
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = to_f<T>(u.e[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 t = to_f2(p[i]);
+      f[2 * i] = t.x, f[2 * i + 1] = t.y;
+    }
+  } else {
+    f[0] = to_f(u.e[0]);
+  }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
   Vec<T, V> u;
+  if constexpr (V % 2 == 0) {
+    auto* q = reinterpret_cast<typename Two<T>::type*>(&u);
 #pragma unroll
-  for (int i = 0; i < V; ++i) u.e[i] = from_f<T>(f[i]);
+    for (int i = 0; i < V / 2; ++i) from_f2(f[2 * i], f[2 * i + 1], q + i);
+  } else {
+    from_f(f[0], &u.e[0]);
+  }
   *reinterpret_cast<Vec<T, V>*>(p) = u;
+}
+
+// V floats of a weight array, 16 bytes at a time where V allows, or `fill` without one.
+template <int V>
+__device__ __forceinline__ void load_weight(const float* p, int c, float fill, float (&f)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = fill;
+    return;
+  }
+  p += c;
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+      f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = __ldg(p + i);
+  }
 }
 
 __device__ __forceinline__ float gate_act(float g, int act) {
@@ -62,174 +108,203 @@ __device__ __forceinline__ float gate_act(float g, int act) {
   return act == kGateSilu ? (s == 0.f ? s : g * s) : s;
 }
 
-// Sum over the L lanes of a row (L <= 32), or over the block (L = 0, `red` of 32 floats).
+// Sum over a row's lanes: L of one warp, or for L = 0 `warps` whole warps that meet at the
+// named barrier `bar` and leave their sums in `red`.
 template <int L>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+__device__ __forceinline__ float row_sum(float v, float* red, int warps, int bar) {
 #pragma unroll
   for (int o = (L ? L : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if constexpr (L == 0) {
-    __syncthreads();  // the previous sum has been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
+    const int w = (threadIdx.x >> 5) % warps;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");  // the last sum has been read
+    if ((threadIdx.x & 31) == 0) red[w] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
     v = 0.f;
-    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) v += red[i];
+    for (int i = 0; i < warps; ++i) v += red[i];
   }
   return v;
 }
 
-// L lanes per row (0: the whole block), N vectors of V elements per lane. Channel of vector
-// n of lane l: (n * lanes + l) * V.
-template <typename T, int V, int L, int N>
-__global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(const NormArgs a) {
-  __shared__ float red[32];
-  const int lanes = L ? L : blockDim.x;
-  const int lane = threadIdx.x % lanes;
-  const long long per_block = blockDim.x / lanes;
+// A row is held by L lanes of a warp, or (L = 0) by `row_warps` whole warps, N vectors of V
+// elements per lane: vector n of lane l starts at channel (n * lanes + l) * V. Each group of
+// lanes walks over rows, and the next row's loads are issued before this row is worked on, so
+// that memory is not idle behind the sums that a row waits for. A lane with one vector keeps
+// its two weight vectors in registers throughout.
+template <typename T, int V, int L, int N, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_kernel(const NormArgs a, int row_warps) {
+  __shared__ float red_all[32];
+  const int lanes = L ? L : row_warps * 32;
+  const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+  float* red = red_all + (L ? 0 : group * row_warps);
+  const int bar = 1 + (L ? 0 : group);
+  const int groups = blockDim.x / lanes;
+  const long long step = static_cast<long long>(gridDim.x) * groups;
   const float inv_c = 1.f / static_cast<float>(a.C);
   const T* x = static_cast<const T*>(a.x);
   const T* y = static_cast<const T*>(a.y);
   const T* gate = static_cast<const T*>(a.gate);
-  const T* mscale = static_cast<const T*>(a.mscale);
-  const T* mshift = static_cast<const T*>(a.mshift);
-  T* out = static_cast<T*>(a.out);
-  T* norm = static_cast<T*>(a.norm);
 
-  for (long long row0 = blockIdx.x * per_block; row0 < a.rows; row0 += gridDim.x * per_block) {
-    const long long row = row0 + threadIdx.x / lanes;
-    const bool live = row < a.rows;  // the lanes of a row past the end take part in the shuffles only
-    float r[N][V];
+  bool in[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) in[n] = (n * lanes + lane) * V < a.C;
+  float ka[V], kw[V];
+  if constexpr (N == 1) {
+    load_weight<V>(a.a, in[0] ? lane * V : 0, 1.f, ka);
+    load_weight<V>(a.w, in[0] ? lane * V : 0, 1.f, kw);
+  }
+
+  Vec<T, V> xn[N] = {}, yn[N] = {};  // the next row, zeros past its end
+  auto fetch = [&](long long row) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int c = (n * lanes + lane) * V;
-      if (live && c < a.C)
-        load<T, V>(x + row * a.xs + c, r[n]);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[n][i] = 0.f;
+      if (!in[n]) continue;
+      xn[n] = load<T, V>(x + row * a.xs + c);
+      if (y) yn[n] = load<T, V>(y + row * a.ys + c);
     }
+  };
+  // Of a row's values: v -> (v - mean) * rstd as v * mul + add.
+  auto statistics = [&](const float(&f)[N][V], int kind, float eps, float* mul, float* add) {
+    float mean = 0.f;
+    *mul = 1.f, *add = 0.f;
+    if (kind == kNormNone) return;
+    if (kind == kNormLayer) {
+      float s = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += f[n][i];
+      mean = row_sum<L>(s, red, row_warps, bar) * inv_c;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!in[n]) continue;
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += (f[n][i] - mean) * (f[n][i] - mean);
+    }
+    *mul = rsqrtf(row_sum<L>(s, red, row_warps, bar) * inv_c + eps);
+    *add = -mean * *mul;
+  };
+  // All lanes of a warp take as many steps as its first group, for the shuffles: a group
+  // whose row lies past the end works on an old row (or zeros) and stores nothing.
+  long long row = static_cast<long long>(blockIdx.x) * groups + group;
+  long long row0 = L ? static_cast<long long>(blockIdx.x) * groups + (threadIdx.x & ~31) / lanes : row;
+  if (row < a.rows) fetch(row);
+  for (; row0 < a.rows; row += step, row0 += step) {
+    const bool live = row < a.rows;
+    float r[N][V], b[N][V], mul, add;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      unpack<T, V>(xn[n], r[n]);
+      unpack<T, V>(yn[n], b[n]);
+    }
+    if (row + step < a.rows) fetch(row + step);
     if (y) {
-      float b[N][V];
+      const T* grow = nullptr;
+      if (gate && live) grow = gate + (a.rows_per_gate == 1 ? row : row / a.rows_per_gate) * a.gs;
+      statistics(b, a.post, a.post_eps, &mul, &add);
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         const int c = (n * lanes + lane) * V;
-        if (live && c < a.C)
-          load<T, V>(y + row * a.ys + c, b[n]);
-        else
+        if (!in[n]) continue;
+        if constexpr (N > 1) load_weight<V>(a.a, c, 1.f, ka);
 #pragma unroll
-          for (int i = 0; i < V; ++i) b[n][i] = 0.f;
-      }
-      float mean = 0.f, rstd = 1.f;
-      if (a.post == kNormLayer) {
-        float s = 0.f;
+        for (int i = 0; i < V; ++i) b[n][i] = (b[n][i] * mul + add) * ka[i];
+        if (a.b) {
+          float kb[V];
+          load_weight<V>(a.b, c, 0.f, kb);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-          for (int i = 0; i < V; ++i) s += b[n][i];
-        mean = row_sum<L>(s, red) * inv_c;
-      }
-      if (a.post != kNormNone) {
-        float s = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-          if ((n * lanes + lane) * V < a.C)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s += (b[n][i] - mean) * (b[n][i] - mean);
-        rstd = rsqrtf(row_sum<L>(s, red) * inv_c + a.post_eps);
-      }
-      const T* grow = gate && live ? gate + row / a.rows_per_gate * a.gs : nullptr;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int c = (n * lanes + lane) * V;
-        if (!live || c >= a.C) continue;
-        float g[V];
+          for (int i = 0; i < V; ++i) b[n][i] += kb[i];
+        }
         if (grow) {
-          load<T, V>(grow + c, g);
+          float g[V];
+          unpack<T, V>(load<T, V>(grow + c), g);
+          if (a.act != kGateLinear) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) g[i] = gate_act(g[i], a.act);
+            for (int i = 0; i < V; ++i) g[i] = gate_act(g[i], a.act);
+          }
+#pragma unroll
+          for (int i = 0; i < V; ++i) b[n][i] *= g[i];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float v = (b[n][i] - mean) * rstd;
-          if (a.a) v *= __ldg(a.a + c + i);
-          if (a.b) v += __ldg(a.b + c + i);
-          r[n][i] += grow ? g[i] * v : v;
-        }
+        for (int i = 0; i < V; ++i) r[n][i] += b[n][i];
       }
     }
-    if (out && live) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int c = (n * lanes + lane) * V;
-        if (c < a.C) store<T, V>(out + row * a.os + c, r[n]);
-      }
-    }
-    if (!norm) continue;
-    float mean = 0.f, rstd = 1.f;
-    if (a.pre == kNormLayer) {
-      float s = 0.f;
+    if (a.out && live) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += r[n][i];
-      mean = row_sum<L>(s, red) * inv_c;
+        if (in[n]) store<T, V>(static_cast<T*>(a.out) + row * a.os + (n * lanes + lane) * V, r[n]);
     }
-    if (a.pre != kNormNone) {
-      float s = 0.f;
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if ((n * lanes + lane) * V < a.C)
-#pragma unroll
-          for (int i = 0; i < V; ++i) s += (r[n][i] - mean) * (r[n][i] - mean);
-      rstd = rsqrtf(row_sum<L>(s, red) * inv_c + a.pre_eps);
-    }
-    const long long mrow = live ? row / a.rows_per_mod * a.ms : 0;
+    if (!a.norm) continue;
+    statistics(r, a.pre, a.pre_eps, &mul, &add);
+    if (!live) continue;
+    const long long mrow = (a.mscale || a.mshift) ? row / a.rows_per_mod * a.ms : 0;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int c = (n * lanes + lane) * V;
-      if (!live || c >= a.C) continue;
-      float m[V];
+      if (!in[n]) continue;
+      if constexpr (N > 1) load_weight<V>(a.w, c, 1.f, kw);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float v = (r[n][i] - mean) * rstd;
-        if (a.w) v *= __ldg(a.w + c + i);
-        if (a.wb) v += __ldg(a.wb + c + i);
-        r[n][i] = v;
+      for (int i = 0; i < V; ++i) r[n][i] = (r[n][i] * mul + add) * kw[i];
+      if (a.wb) {
+        float kb[V];
+        load_weight<V>(a.wb, c, 0.f, kb);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[n][i] += kb[i];
       }
-      if (mscale) {
-        load<T, V>(mscale + mrow + c, m);
+      float m[V];
+      if (a.mscale) {
+        unpack<T, V>(load<T, V>(static_cast<const T*>(a.mscale) + mrow + c), m);
 #pragma unroll
         for (int i = 0; i < V; ++i) r[n][i] += r[n][i] * m[i];
       }
-      if (mshift) {
-        load<T, V>(mshift + mrow + c, m);
+      if (a.mshift) {
+        unpack<T, V>(load<T, V>(static_cast<const T*>(a.mshift) + mrow + c), m);
 #pragma unroll
         for (int i = 0; i < V; ++i) r[n][i] += m[i];
       }
-      store<T, V>(norm + row * a.ns + c, r[n]);
+      store<T, V>(static_cast<T*>(a.norm) + row * a.ns + c, r[n]);
     }
   }
 }
 
-template <typename T, int V, int L, int N>
-cudaError_t launch(const NormArgs& a, int threads, int num_sms, cudaStream_t s) {
-  const long long per_block = L ? threads / L : 1;
-  const long long blocks = std::min<long long>((a.rows + per_block - 1) / per_block, num_sms * (L ? 8LL : 4LL));
-  norm_kernel<T, V, L, N><<<static_cast<unsigned>(blocks), threads, 0, s>>>(a);
+template <typename T, int V, int L, int N, int THREADS = 256, int BLOCKS = 1>
+cudaError_t launch(const NormArgs& a, int row_warps, int num_sms, cudaStream_t s) {
+  auto fn = norm_kernel<T, V, L, N, THREADS, BLOCKS>;
+  const int groups = THREADS / (L ? L : row_warps * 32);
+  const int threads = groups * (L ? L : row_warps * 32);
+  // As many blocks as fit at once (the same on every sm_100 GPU), each walking over its rows.
+  static std::atomic<int> fit[33];  // by row_warps
+  int per_sm = fit[row_warps].load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, 0);
+    if (e != cudaSuccess) return e;
+    fit[row_warps].store(per_sm, std::memory_order_relaxed);
+  }
+  const long long blocks =
+      std::min<long long>((a.rows + groups - 1) / groups, static_cast<long long>(num_sms) * per_sm);
+  fn<<<static_cast<unsigned>(blocks), threads, 0, s>>>(a, row_warps);
   return cudaGetLastError();
 }
 
+// Few vectors a lane: they and the next row's are held in registers, and it is rows in flight
+// that hide the wait for memory and for the sums.
 template <typename T, int V>
 cudaError_t by_width(const NormArgs& a, int num_sms, cudaStream_t s) {
   const int n = (a.C + V - 1) / V;  // vectors in a row
-  if (n <= 8) return launch<T, V, 8, 1>(a, 256, num_sms, s);
-  if (n <= 16) return launch<T, V, 16, 1>(a, 256, num_sms, s);
-  if (n <= 32) return launch<T, V, 32, 1>(a, 256, num_sms, s);
-  if (n <= 64) return launch<T, V, 32, 2>(a, 256, num_sms, s);
-  if (n <= 128) return launch<T, V, 32, 4>(a, 256, num_sms, s);
-  if (n <= 1024) return launch<T, V, 0, 1>(a, (n + 31) / 32 * 32, num_sms, s);
-  if constexpr (V < 8) {  // n is at most 8192 / V
-    if (n <= 2048) return launch<T, V, 0, 2>(a, 1024, num_sms, s);
-    return launch<T, V, 0, 8>(a, 1024, num_sms, s);
+  if (n <= 8) return launch<T, V, 8, 1, 256, 4>(a, 1, num_sms, s);
+  if (n <= 16) return launch<T, V, 16, 1, 256, 4>(a, 1, num_sms, s);
+  if (n <= 32) return launch<T, V, 32, 1, 256, 4>(a, 1, num_sms, s);
+  if (n <= 48) return launch<T, V, 16, 3>(a, 1, num_sms, s);
+  if (n <= 64) return launch<T, V, 32, 2>(a, 1, num_sms, s);
+  if (n <= 256) return launch<T, V, 0, 1, 256, 4>(a, (n + 31) / 32, num_sms, s);
+  if (n <= 512) return launch<T, V, 0, 2, 256, 2>(a, (n + 63) / 64, num_sms, s);
+  if (n <= 1024) return launch<T, V, 0, 4>(a, (n + 127) / 128, num_sms, s);
+  // n is at most 8192 / V
+  if constexpr (V < 8) {
+    if (n <= 4096) return launch<T, V, 0, 4, 1024>(a, 32, num_sms, s);
+    return launch<T, V, 0, 8, 1024>(a, 32, num_sms, s);
   }
   return cudaErrorInvalidValue;
 }
