@@ -8,11 +8,7 @@
 // never below the prefix. So a mask is two comparisons, made only in tiles that some row's
 // interval ends in, and tiles that no row sees are not loaded.
 //
-// Scores are kept as powers of two (x = score * log2 e), capped and biased in fp32:
-//   cap tanh(s / cap) = cap (1 - 2 / (1 + exp(2 s / cap)))
-// which is exact to a few units of 2^-24 cap; beyond a cap of 256, where that is no longer
-// small beside the score, small arguments take the odd series of tanh instead.
-// The weights 2^(x - max) are rounded to the tensors' type for the second product, as the
+// Scores are kept as powers of two (x = score * log2 e), capped and biased in fp32. The weights 2^(x - max) are rounded to the tensors' type for the second product, as the
 // matrix instructions take no wider operand; their sum is taken before that rounding.
 //
 // Keys and values beyond a document's keys in use are filled with zeros as they are staged,
@@ -23,9 +19,7 @@
 // joined at the end. Either may share its keys out over a cluster of CTAs, whose partial
 // results are joined through distributed shared memory, so no workspace is needed and the
 // order of the sums is fixed.
-#include "tokens.h"
-
-#include <atomic>
+#include "attn_common.cuh"
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -39,7 +33,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kStages = 3;
-constexpr float kSeriesCap = 256.f;
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -96,16 +89,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-__device__ __forceinline__ float capped(float s, const AttnArgs& a) {
-  const float u = s * a.cap_arg;
-  if (a.cap_log2 > kSeriesCap * 1.44269504f && fabsf(u) < 0.3f) {
-    // tanh u = u - u^3/3 + 2u^5/15 - 17u^7/315 + 62u^9/2835; the next term is below 2^-24 u
-    const float z = u * u;
-    return a.cap_log2 * u * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835)))));
-  }
-  return a.cap_log2 - __fdividef(2.f * a.cap_log2, 1.f + exp2_fast(u * 2.88539008f));
 }
 
 template <int DP, bool FEW>
@@ -258,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = capped(s[n][e], a);
+        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped(s[n][e], a);
     } else {
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
@@ -423,17 +406,9 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
 template <typename T, int DP, bool FEW>
 cudaError_t launch(const AttnArgs& a, int cluster, cudaStream_t s) {
   auto fn = attn_mma_kernel<T, DP, FEW>;
-  static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel has its attributes
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static AttrOnce once;
+  const cudaError_t e = once.set(reinterpret_cast<const void*>(fn), Layout<DP, FEW>::kBytes, true);
   if (e != cudaSuccess) return e;
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (!(ready.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DP, FEW>::kBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    ready.fetch_or(bit, std::memory_order_release);
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.num_items) * cluster, a.kv_heads);
   cfg.blockDim = dim3(kThreads);

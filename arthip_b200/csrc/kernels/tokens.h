@@ -83,8 +83,8 @@ constexpr int kAttnMaxAxes = 3;
 struct AttnDoc {
   int q0, nq, k0, nk, prefix;
 };
-// A block of rows of one document. A row is a query token and one of the query heads that
-// share a key head: row = token * group + head in group.
+// A block of rows of one document, from row row0. A row is a query token and one of the query
+// heads that share a key head: row = token * group + head in group.
 struct AttnItem {
   int doc, row0;
 };
@@ -115,5 +115,13 @@ constexpr int kMmaRowsWide = 64;  // four warps of 16 rows
 constexpr int kMmaRowsFew = 16;   // 16 rows, the keys shared out over the warps
 constexpr int kMmaKeys = 64;      // keys per tile
 cudaError_t attn_mma_launch(const AttnArgs& a, int dtype, bool few_rows, int cluster, cudaStream_t s);
+
+// attn_tc.cu: tcgen05 form. Its items are not rows but query tokens: two tiles of 128, one
+// after the other of one query head, or, for an even group, of the same tokens for two heads.
+constexpr int kTcRows = 128;
+constexpr int kTcKeys = 128;
+inline bool attn_tc_head_pairs(int group) { return group % 2 == 0; }
+inline int attn_tc_item_tokens(int group) { return attn_tc_head_pairs(group) ? kTcRows : 2 * kTcRows; }
+cudaError_t attn_tc_launch(const AttnArgs& a, int dtype, cudaStream_t s, std::string* err);
 
 }  // namespace ah

@@ -149,6 +149,11 @@ bool Overlap(const View& a, const View& b) {
 
 bool Aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Which documents the tcgen05 kernel takes: those that fill more than half of its tiles of 128
+// queries and one tile of keys. At 64 queries and keys (2040 windows, 6 heads of 32) it takes
+// the mma.sync kernel 125 us; at 32400 of both (8 heads of 64) 8.2 ms against 4.4 ms here.
+bool UseTensorMemory(const ah::AttnDoc& doc) { return doc.nq > ah::kTcRows / 2 && doc.nk >= ah::kTcKeys; }
+
 View Floats(const float* p, int64_t n) { return View{p, 1, 0, 1, 0, 2 * n}; }
 
 }  // namespace
@@ -170,8 +175,8 @@ struct ah_attn {
   int device = 0, num_sms = 0, dtype = 0;
   ah::AttnArgs args;
   int64_t q_total = 0, k_total = 0;
-  DeviceBuffer docs, few, wide, slopes;
-  int n_few = 0, n_wide = 0, few_cluster = 1, wide_cluster = 1;
+  DeviceBuffer docs, few, wide, tc, slopes, status;
+  int n_few = 0, n_wide = 0, n_tc = 0, few_cluster = 1, wide_cluster = 1;
 };
 
 extern "C" {
@@ -450,20 +455,26 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
     a.score_mul = static_cast<float>(d->scale * kLog2e);
   }
   // Blocks of rows, those with the most keys first, so that the last ones to start are short.
-  std::vector<ah::AttnItem> few, wide;
+  std::vector<ah::AttnItem> few, wide, tc;
   int few_tiles = 0, wide_tiles = 0;
   std::vector<int> order(docs);
   for (int i = 0; i < docs; ++i) order[i] = i;
   std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return table[i].nk > table[j].nk; });
   for (int i : order) {
-    const int rows = table[i].nq * group, tiles = (table[i].nk + ah::kMmaKeys - 1) / ah::kMmaKeys;
+    const ah::AttnDoc& doc = table[i];
+    if (UseTensorMemory(doc)) {
+      const int step = ah::attn_tc_item_tokens(group);
+      for (int r = (doc.nq - 1) / step * step; r >= 0; r -= step) tc.push_back({i, r});  // causal: longest first
+      continue;
+    }
+    const int rows = doc.nq * group, tiles = (doc.nk + ah::kMmaKeys - 1) / ah::kMmaKeys;
     const bool is_few = rows <= ah::kMmaRowsFew;
     const int step = is_few ? ah::kMmaRowsFew : ah::kMmaRowsWide;
     for (int r = 0; r < rows; r += step) (is_few ? few : wide).push_back({i, r});
     int& t = is_few ? few_tiles : wide_tiles;
     if (rows) t = std::max(t, tiles);
   }
-  if (few.size() > (1u << 26) || wide.size() > (1u << 26))
+  if (few.size() + wide.size() + tc.size() > (1u << 26))
     return Fail("attention: more than 2^26 blocks of rows", err, errlen);
   // A cluster of CTAs shares one block's keys while that leaves SMs without work and each CTA
   // at least four tiles.
@@ -474,15 +485,20 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   };
   h->n_few = static_cast<int>(few.size());
   h->n_wide = static_cast<int>(wide.size());
+  h->n_tc = static_cast<int>(tc.size());
   h->few_cluster = cluster(few.size(), few_tiles);
   h->wide_cluster = cluster(wide.size(), wide_tiles);
   cudaError_t e = h->docs.Upload(table.data(), table.size() * sizeof(ah::AttnDoc));
   if (e == cudaSuccess) e = h->few.Upload(few.data(), few.size() * sizeof(ah::AttnItem));
   if (e == cudaSuccess) e = h->wide.Upload(wide.data(), wide.size() * sizeof(ah::AttnItem));
+  if (e == cudaSuccess) e = h->tc.Upload(tc.data(), tc.size() * sizeof(ah::AttnItem));
   if (e == cudaSuccess) e = h->slopes.Upload(bias.data(), bias.size() * sizeof(float));
+  const uint32_t zero = 0;
+  if (e == cudaSuccess) e = h->status.Upload(&zero, sizeof zero);
   if (e != cudaSuccess) return CudaFail("attention plan upload failed", e, err, errlen, 1);
   a.docs = h->docs.as<ah::AttnDoc>();
   a.slopes = h->slopes.as<float>();
+  a.status = h->status.as<uint32_t>();
   *out = h.release();
   return 0;
 } catch (const std::bad_alloc&) {
@@ -526,7 +542,13 @@ int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int e
   a.v_tok = v.tok, a.v_head = v.head, a.o_tok = o.tok, a.o_head = o.head;
   a.q_pos = io->q_positions, a.k_pos = io->k_positions, a.k_lens = io->k_lens;
   cudaError_t e = cudaSuccess;
-  if (h->n_wide) {
+  std::string what = "attention launch failed";
+  if (h->n_tc) {
+    a.items = h->tc.as<ah::AttnItem>();
+    a.num_items = h->n_tc;
+    e = ah::attn_tc_launch(a, h->dtype, s, &what);
+  }
+  if (e == cudaSuccess && h->n_wide) {
     a.items = h->wide.as<ah::AttnItem>();
     a.num_items = h->n_wide;
     e = ah::attn_mma_launch(a, h->dtype, false, h->wide_cluster, s);
@@ -536,7 +558,15 @@ int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int e
     a.num_items = h->n_few;
     e = ah::attn_mma_launch(a, h->dtype, true, h->few_cluster, s);
   }
-  return e == cudaSuccess ? 0 : CudaFail("attention launch failed", e, err, errlen, 2);
+  return e == cudaSuccess ? 0 : CudaFail(what.c_str(), e, err, errlen, 2);
+}
+
+int ah_attn_status(ah_attn* h, uint32_t* status) {
+  if (!h || !status) return 1;
+  DeviceScope scope(h->device);
+  if (scope.error() != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) return 2;
+  if (cudaMemcpy(status, h->args.status, sizeof(uint32_t), cudaMemcpyDeviceToHost) != cudaSuccess) return 2;
+  return cudaMemset(h->args.status, 0, sizeof(uint32_t)) == cudaSuccess ? 0 : 2;
 }
 
 void ah_attn_destroy(ah_attn* h) {

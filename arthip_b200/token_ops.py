@@ -238,3 +238,11 @@ class TokenAttention(_Handle):
         err = _err()
         self._check(self._lib.ah_attn_run(self._h, ctypes.byref(io), stream or None, err, _ERR_LEN), err,
                     "attention run")
+
+    def status(self) -> int:
+        """The device error word (0 = none), read and cleared: a pipeline wait that ran out.
+        Synchronises the device."""
+        st = ctypes.c_uint32(0)
+        if self._lib.ah_attn_status(self._h, ctypes.byref(st)) != 0:
+            raise EngineHarnessError("attention status read failed")
+        return st.value

@@ -332,6 +332,9 @@ int ah_attn_create(int device, const ah_attn_desc* desc, int docs, const int64_t
                    const int64_t* k_offsets, const int64_t* prefix, const float* slopes, ah_attn** out, char* err,
                    int errlen);
 int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int errlen);
+/* Reads and clears the device error word that the tensor-core kernel writes when a pipeline
+ * wait runs out (0 = none; the run's output is then incomplete). Synchronises the device. */
+int ah_attn_status(ah_attn* h, uint32_t* status);
 void ah_attn_destroy(ah_attn* h);
 
 /* Test-only failure-path hook (no counterpart in the reference). For tensor-core conv launches made after the call, in this process:

@@ -45,6 +45,8 @@ cudaError_t cudaMalloc(void** p, size_t n) {
 }
 cudaError_t cudaFree(void* p) { std::free(p); --g_live; return cudaSuccess; }
 cudaError_t cudaMemcpy(void* d, const void* s, size_t n, cudaMemcpyKind) { std::memcpy(d, s, n); return cudaSuccess; }
+cudaError_t cudaMemset(void* d, int v, size_t n) { std::memset(d, v, n); return cudaSuccess; }
+cudaError_t cudaDeviceSynchronize() { return cudaSuccess; }
 const char* cudaGetErrorString(cudaError_t) { return "stand-in error"; }
 cudaError_t cudaGetLastError() { return cudaSuccess; }
 cudaError_t cudaStreamIsCapturing(cudaStream_t, cudaStreamCaptureStatus* c) {
@@ -60,6 +62,7 @@ cudaError_t cudaStreamGetDevice(cudaStream_t s, int* d) {
 namespace ah {
 cudaError_t norm_launch(const NormArgs&, int, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
 cudaError_t rope_launch(const RopeTable&, const RopeArgs&, int, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
+cudaError_t attn_tc_launch(const AttnArgs&, int, cudaStream_t, std::string*) { ++g_launches; return cudaSuccess; }
 cudaError_t attn_mma_launch(const AttnArgs&, int, bool, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
 }
 """

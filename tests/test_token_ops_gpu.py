@@ -254,6 +254,7 @@ def run_attn(qs, ks, hq=4, hk=2, d=64, dtype="fp16", causal=False, prefix=None, 
                           dtype)
     check(out[:nq], ref, bound, dtype, "attention")
     assert (out[nq:] == 7).all()
+    assert op.status() == 0
     op.close()
 
 
