@@ -6,13 +6,21 @@
 //   P = 2^(x - m)  one thread per row; rounded to 16 bits into the columns S was in
 //   O += P V     A from tensor memory, B = V as TMA brought it (MN-major)
 //
-// Two warpgroups work on the two tiles' softmax in turn with the tensor cores: while one
-// tile's S and O products run, the other's exponentials do. A thread holds a whole row of S,
-// so its maximum and sum need no exchange. Warp 8 issues the TMA loads of the key and value
-// tiles into a ring, warp 9 the products; its issue order (O += P V of a tile, then S of the
-// same tile's next keys) makes S's completion stand for O's: a warpgroup that sees S may
-// rescale O. It does so only where a row's maximum has grown by more than 2^8, so in most
-// tiles O stays where it is; weights reach 2^14 at most, which fp16 holds.
+// Keys are taken 128 at a time. Eight warps work on each tile's softmax, 16 rows each, so that
+// each of the SM's four schedulers has four of them: some have exponentials to do while others
+// wait for S, load it or look for its maximum. Four threads share a row (the 16-lane loads of
+// tensor memory give each of them every fourth pair of columns) and find its maximum with two
+// shuffles. Half of the scores are loaded a second time rather than kept, which holds a thread
+// to the 96 registers that 19 warps leave it. Warp 16 issues the TMA loads of key and value
+// tiles into a ring, warps 17 and 18 the products of one tile each.
+//
+// Heads of up to 64 have room for P beside S: S of the next keys is computed as soon as this
+// one has been loaded into registers, and a softmax warp never waits for the round trip
+// through the tensor cores. For wider heads P takes the place of S, and S of the next keys
+// follows O += P V; there the two tiles' warps work in turn.
+//
+// O is rescaled only where a row's maximum has grown by more than 2^8, so in most steps it
+// stays where it is; weights reach 2^14 at most, which fp16 holds.
 //
 // Masks, caps and biases are as in attn_mma.cu. Values behind a document's keys in use are
 // written over with zeros in shared memory before the product that reads them, and whole
@@ -37,7 +45,8 @@ struct AttnTcArgs {
 
 namespace attn_tc {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 608;
+constexpr int kLoadWarp = 16, kProductWarp = 17;  // and the next; softmax: 0-15
 constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr float kWeightShift = 6.f;     // weights are 2^(x - m + 6): a wider range above fp16's smallest
 constexpr float kRescaleAt = 8.f;
@@ -50,7 +59,12 @@ struct Smem {
   static constexpr int kQ = 0;
   static constexpr int kRing = kQ + 2 * kTile;
   static constexpr int kPos = kRing + kSlots * kTile;  // key positions: [2 tiles][2 buffers][axes][128]
-  static constexpr int kBars = kPos + 2 * 2 * kAttnMaxAxes * kTcKeys * 4;
+  static constexpr int kSums = kPos + 2 * 2 * kAttnMaxAxes * kTcKeys * 4;  // [2 tiles][128]
+  static constexpr int kBars = kSums + 2 * kTcRows * 4;
+  // tensor memory columns
+  static constexpr bool kOwnP = NCH == 1;  // P has columns of its own
+  static constexpr int kCols = NCH * 64;   // of O
+  static constexpr int kColO = 256, kColP = kOwnP ? 384 : 0, kStrideP = kOwnP ? 64 : 128;
   static constexpr int kBytes = kBars + 256 + 1024;    // and room to align to 1024
 };
 
@@ -78,6 +92,23 @@ constexpr bool kIsBf16 = false;
 template <>
 constexpr bool kIsBf16<__nv_bfloat16> = true;
 
+// The weights 2^(u * mul + base) of a thread's share of 64 columns (16-lane layout: registers
+// 4k, 4k + 1 are of its first row, 4k + 2, 4k + 3 of its second), packed to 16 bits, and their
+// sums added to `sum`.
+template <typename T>
+__device__ __forceinline__ void weights32(const uint32_t (&u)[32], uint64_t mul, const uint64_t (&base)[2],
+                                          uint32_t (&w)[16], uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t x =
+        ptx::fma_f2(ptx::pack_f2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), mul, base[i & 1]);
+    const float2 v = ptx::unpack_f2(x);
+    const float p0 = exp2_fast(v.x), p1 = exp2_fast(v.y);
+    sum[i & 1] = ptx::add_f2(sum[i & 1], ptx::pack_f2(p0, p1));
+    w[i] = pack2<T>(p0, p1);
+  }
+}
+
 template <typename T, int NCH, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ AttnTcArgs args) {
   using L = Smem<NCH>;
@@ -87,11 +118,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* full = bars;                 // [kSlots] a K or V tile has landed
   uint64_t* empty = full + L::kSlots;    // [kSlots] the products that read it are done
-  uint64_t* s_full = empty + L::kSlots;  // [2] S of a tile (and the O before it) is complete
-  uint64_t* p_ready = s_full + 2;        // [2] its weights are in tensor memory (a count of 4 warps)
-  uint64_t* q_full = p_ready + 2;
-  uint64_t* drained = q_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* s_full = empty + L::kSlots;  // [2 tiles] S of a step is complete (wide heads: and O before it)
+  uint64_t* s_free = s_full + 2;         // [2] it has been loaded (a count of 8 warps)
+  uint64_t* p_ready = s_free + 2;        // [2] its weights are in tensor memory (8 warps)
+  uint64_t* o_done = p_ready + 2;        // [2] and have been added to O
+  uint64_t* q_full = o_done + 2;
+  uint64_t* drained = q_full + 1;        // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -119,18 +152,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       ptx::mbar_init(ptx::smem_u32(full + i), 1);
-      ptx::mbar_init(ptx::smem_u32(empty + i), 1);
+      ptx::mbar_init(ptx::smem_u32(empty + i), 2);
     }
     for (int g = 0; g < 2; ++g) {
       ptx::mbar_init(ptx::smem_u32(s_full + g), 1);
-      ptx::mbar_init(ptx::smem_u32(p_ready + g), 4);
+      ptx::mbar_init(ptx::smem_u32(s_free + g), 8);
+      ptx::mbar_init(ptx::smem_u32(p_ready + g), 8);
+      ptx::mbar_init(ptx::smem_u32(o_done + g), 1);
     }
     ptx::mbar_init(ptx::smem_u32(q_full), 1);
     ptx::mbar_init(ptx::smem_u32(drained), 1);
+    ptx::mbar_init(ptx::smem_u32(drained + 1), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kProductWarp) {
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
     ptx::tmem_relinquish();
   }
@@ -140,9 +176,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   const uint32_t tmem = *tmem_slot;
   int never_abort = 0;
 
-  if (warp == 8) {
+  if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ loads
-    if (lane == 0) {
+    if (ptx::elect_one()) {
       ptx::prefetch_tensormap(&args.q);
       ptx::prefetch_tensormap(&args.k);
       ptx::prefetch_tensormap(&args.v);
@@ -157,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       for (; issued < 2 * ntiles; ++issued) {  // K and V of each tile in turn
         const int slot = issued % L::kSlots, use = issued / L::kSlots;
-        if (!ptx::mbar_wait(ptx::smem_u32(empty + slot), (use & 1) ^ 1, abort_flag)) break;
+        if (!ptx::mbar_wait_short(ptx::smem_u32(empty + slot), (use & 1) ^ 1, abort_flag)) break;
         const uint32_t fb = ptx::smem_u32(full + slot);
         ptx::mbar_arrive_expect_tx(fb, L::kTile);
         const CUtensorMap* map = issued & 1 ? &args.v : &args.k;
@@ -166,252 +202,324 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                            doc.k0 + (issued >> 1) * kTcKeys, kvh);
       }
       // Nothing may be in flight when the CTA ends, which after a wait that ran out it might.
-      if (ntiles > 0) ptx::mbar_wait(ptx::smem_u32(q_full), 0, &never_abort);
+      if (ntiles > 0) ptx::mbar_wait_short(ptx::smem_u32(q_full), 0, &never_abort);
       for (int i = max(0, issued - L::kSlots); i < issued; ++i)
-        ptx::mbar_wait(ptx::smem_u32(full + i % L::kSlots), (i / L::kSlots) & 1, &never_abort);
+        ptx::mbar_wait_short(ptx::smem_u32(full + i % L::kSlots), (i / L::kSlots) & 1, &never_abort);
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp >= kProductWarp) {
     // --------------------------------------------------------------- products
-    const int ksteps_q = (a.head_dim + 15) / 16;
-    const uint32_t n_out = ksteps_q * 16;
-    auto ring = [&](int seq) { return ptx::smem_u32(smem + L::kRing + seq % L::kSlots * L::kTile); };
-    auto await = [&](uint64_t* bar, int parity) {  // the same answer in all lanes
-      return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort_flag)) != 0;
+    // The issue loops hold nothing but additions of constants: descriptors and counts are made
+    // once, as one thread's instructions between two products are what would bound them.
+    const int g = warp - kProductWarp;
+    const int ksteps = (a.head_dim + 15) / 16;
+    const uint32_t idesc_s = ptx::idesc_16_f32(kIsBf16<T>, false, kTcRows, 0);
+    const uint32_t idesc_o = ptx::idesc_16_f32(kIsBf16<T>, true, kTcRows, ksteps * 16);
+    constexpr uint32_t kHi = ptx::desc_hi(1024, 2);
+    const uint32_t ring0 = ptx::smem_u32(smem + L::kRing);
+    const uint32_t q_lo = ptx::desc_lo(ptx::smem_u32(smem + L::kQ)) + g * (L::kTile >> 4);
+    const uint32_t k_lo = ptx::desc_lo(ring0), v_lo = ptx::desc_lo_mn(ring0, kChunkBytes);
+    const uint32_t ts = tmem + g * 128, to = tmem + L::kColO + g * L::kCols;
+    const uint32_t tp = tmem + L::kColP + g * L::kStrideP;
+    const int n = tiles[g];
+    auto slot_words = [&](int seq) { return static_cast<uint32_t>(seq % L::kSlots * (L::kTile >> 4)); };
+    auto await = [&](uint64_t* bar, int parity) {
+      return ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag);
     };
     auto wait_full = [&](int seq) { return await(full + seq % L::kSlots, (seq / L::kSlots) & 1); };
-    auto seen = [&](int g, int j) { return min(kTcKeys, hi_top[g] - j * kTcKeys); };  // keys of tile j
-    auto issue_s = [&](int g, int j) {
-      const uint32_t q = ptx::smem_u32(smem + L::kQ + g * L::kTile), k = ring(2 * j);
-      const uint32_t idesc = ptx::idesc_16_f32(kIsBf16<T>, false, kTcRows, (seen(g, j) + 15) / 16 * 16);
-      for (int s = 0; s < ksteps_q; ++s) {
-        const uint32_t off = (s >> 2) * kChunkBytes + (s & 3) * 32;
-        ptx::mma_f16_ss(tmem + g * 128, ptx::smem_desc(q + off, 2, 1024), ptx::smem_desc(k + off, 2, 1024), idesc,
-                        s > 0);
+    auto release = [&](int seq) { ptx::mma_commit(ptx::smem_u32(empty + seq % L::kSlots)); };
+    auto key_steps = [&](int j) {  // 16s of keys of tile j that some row sees
+      return (min(kTcKeys, hi_top[g] - j * kTcKeys) + 15) / 16;
+    };
+    auto issue_s = [&](int j) {
+      const uint32_t k = k_lo + slot_words(2 * j);
+      const uint32_t idesc = idesc_s | static_cast<uint32_t>(key_steps(j)) << 18;  // N / 8
+#pragma unroll
+      for (int s = 0; s < 4 * NCH; ++s) {
+        const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
+        if (s < ksteps) ptx::mma_f16_ss2(ts, q_lo + off, kHi, k + off, kHi, idesc, s > 0);
       }
     };
-    auto issue_o = [&](int g, int j) {
-      const uint32_t v = ring(2 * j + 1);
-      const uint32_t idesc = ptx::idesc_16_f32(kIsBf16<T>, true, kTcRows, n_out);
-      const int steps = (seen(g, j) + 15) / 16;
-      for (int s = 0; s < steps; ++s)
-        ptx::mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + s * 8,
-                        ptx::smem_desc_mn128(v + s * 2048, kChunkBytes, 1024), idesc, j > 0 || s > 0);
+    auto issue_o = [&](int j) {
+      const uint32_t v = v_lo + slot_words(2 * j + 1), more = j > 0;
+      const int steps = key_steps(j);
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < steps) ptx::mma_f16_ts(to, tp + s * 8, v + s * 128, kHi, idesc_o, s > 0 ? 1u : more);
     };
-    bool ok = true;
-    if (ntiles > 0) {
-      ok = await(q_full, 0) && wait_full(0);
-      ptx::tc_fence_after();
-      if (ok && lane == 0) {
-        for (int g = 0; g < 2; ++g)
-          if (tiles[g] > 0) {
-            issue_s(g, 0);
+    auto clear_values = [&](int j) {  // zeros behind the keys in use, to the end of their 16
+      const int used = klen - j * kTcKeys;
+      if (used >= kTcKeys || used % 16 == 0) return;
+      uint8_t* v = smem + L::kRing + (2 * j + 1) % L::kSlots * L::kTile;
+      const int words = (16 - used % 16) * 8;  // of 16 bytes, per chunk
+      for (int i = 0; i < NCH * words; ++i)
+        *reinterpret_cast<uint4*>(v + i / words * kChunkBytes + used * 128 + i % words * 16) = make_uint4(0, 0, 0, 0);
+      ptx::fence_proxy_async_smem();
+    };
+    if (ntiles > 0 && ptx::elect_one()) {
+      bool ok = (n == 0 || await(q_full, 0)) && wait_full(0);
+      if (ok) {
+        ptx::tc_fence_after();
+        if (n > 0) issue_s(0);
+        ptx::mma_commit(ptx::smem_u32(s_full + g));
+        release(0);
+      }
+      for (int j = 0; j < ntiles && ok; ++j) {
+        const bool last = j + 1 == ntiles;
+        if constexpr (L::kOwnP) {
+          if (!last) {
+            ok = wait_full(2 * j + 2) && (j + 1 >= n || await(s_free + g, j & 1));
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (j + 1 < n) {
+              issue_s(j + 1);
+              ptx::mma_commit(ptx::smem_u32(s_full + g));
+            }
+            release(2 * j + 2);
+          }
+          ok = wait_full(2 * j + 1);
+          if (!ok) break;
+          clear_values(j);
+          if (j < n) {
+            ok = await(p_ready + g, j & 1);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            issue_o(j);
+            ptx::mma_commit(ptx::smem_u32(o_done + g));
+          }
+          release(2 * j + 1);
+        } else {
+          ok = wait_full(2 * j + 1) && (last || wait_full(2 * j + 2));
+          if (!ok) break;
+          clear_values(j);
+          if (j < n) {
+            ok = await(p_ready + g, j & 1);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            issue_o(j);
+            if (j + 1 < n) issue_s(j + 1);
             ptx::mma_commit(ptx::smem_u32(s_full + g));
           }
-        ptx::mma_commit(ptx::smem_u32(empty + 0));
-      }
-      __syncwarp();
-    }
-    for (int j = 0; j < ntiles && ok; ++j) {
-      bool have_v = false, have_k = false;
-      for (int g = 0; g < 2 && ok; ++g) {
-        if (j >= tiles[g]) continue;
-        if (!have_v) {
-          ok = wait_full(2 * j + 1);
-          have_v = true;
-          const int used = klen - j * kTcKeys;
-          if (ok && used < kTcKeys && used % 16) {  // zeros behind the keys in use, to the end of their step
-            uint8_t* v = smem + L::kRing + (2 * j + 1) % L::kSlots * L::kTile;
-            const int words = (16 - used % 16) * 8;  // of 16 bytes, per chunk
-            for (int i = lane; i < NCH * words; i += 32)
-              *reinterpret_cast<uint4*>(v + i / words * kChunkBytes + used * 128 + i % words * 16) =
-                  make_uint4(0, 0, 0, 0);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-          }
+          release(2 * j + 1);
+          if (!last) release(2 * j + 2);
         }
-        ok = ok && await(p_ready + g, j & 1);
-        const bool more = j + 1 < tiles[g];
-        if (ok && more && !have_k) {
-          ok = wait_full(2 * j + 2);
-          have_k = true;
-        }
-        if (!ok) break;
-        ptx::tc_fence_after();
-        if (lane == 0) {
-          issue_o(g, j);
-          if (more) issue_s(g, j + 1);
-          ptx::mma_commit(ptx::smem_u32(s_full + g));
-        }
-        __syncwarp();
       }
-      if (ok && lane == 0) {
-        ptx::mma_commit(ptx::smem_u32(empty + (2 * j + 1) % L::kSlots));
-        if (j + 1 < ntiles) ptx::mma_commit(ptx::smem_u32(empty + (2 * j + 2) % L::kSlots));
-      }
-      __syncwarp();
-    }
-    // No product may be running when tensor memory is freed.
-    if (lane == 0 && ntiles > 0) {
-      ptx::mma_commit(ptx::smem_u32(drained));
-      ptx::mbar_wait(ptx::smem_u32(drained), 0, &never_abort);
+      // No product may be running when tensor memory is freed.
+      ptx::mma_commit(ptx::smem_u32(drained + g));
+      ptx::mbar_wait_short(ptx::smem_u32(drained + g), 0, &never_abort);
     }
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax
-    const int g = warp >> 2;
-    const int r = threadIdx.x & 127;  // row of the tile = lane of tensor memory
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-    const uint32_t ts = tmem + lanes + g * 128, to = tmem + lanes + 256 + g * 128;
+    const int g = warp >> 3;
+    const int row16 = (warp & 3) * 32 + (warp >> 2 & 1) * 16;  // this warp's rows of the tile
+    const int t4 = lane & 3;
+    const uint32_t lanes = static_cast<uint32_t>(row16) << 16;
+    const uint32_t ts = tmem + lanes + g * 128;
+    const uint32_t to = tmem + lanes + L::kColO + g * L::kCols;
+    const uint32_t tp = tmem + lanes + L::kColP + g * L::kStrideP;
     const int n = tiles[g];
-    const bool mine = r < ntok[g];
-    const int tok = tok0[g] + min(r, max(ntok[g] - 1, 0));
-    const int hi = n ? hi_of(tok) : 0;
     const int hi_low = n ? hi_of(tok0[g]) : 0;
-    float* pos_all = reinterpret_cast<float*>(smem + L::kPos) + g * 2 * kAttnMaxAxes * kTcKeys;
-    float slope[kAttnMaxAxes], qpos[kAttnMaxAxes], kpos[kAttnMaxAxes];
-    auto fetch_pos = [&](int j) {  // one key of tile j per thread
-      const int key = j * kTcKeys + r;
+    int hi[2];
+    float slope[kAttnMaxAxes], qpos[2][kAttnMaxAxes];
 #pragma unroll
-      for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-        if (ax < a.axes) kpos[ax] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
-    };
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
-        slope[ax] = ax < a.axes && n ? a.slopes[head[g] * a.axes + ax] : 0.f;
-        qpos[ax] = ax < a.axes && n ? a.q_pos[ax * a.q_total + doc.q0 + tok] : 0.f;
-      }
-      if (n) fetch_pos(0);
-    }
-    const float mul = CAP || BIAS ? 1.f : a.score_mul;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      float* pos = pos_all + (j & 1) * kAttnMaxAxes * kTcKeys;
+    for (int e = 0; e < 2; ++e) {  // this thread's two rows, row16 + lane / 4 and + 8
+      const int tok = tok0[g] + min(row16 + (lane >> 2) + 8 * e, max(ntok[g] - 1, 0));
+      hi[e] = n ? hi_of(tok) : 0;
       if constexpr (BIAS) {
 #pragma unroll
-        for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-          if (ax < a.axes) pos[ax * kTcKeys + r] = kpos[ax];
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
-        if (j + 1 < n) fetch_pos(j + 1);
+        for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
+          slope[ax] = ax < a.axes && n ? a.slopes[head[g] * a.axes + ax] : 0.f;
+          qpos[e][ax] = ax < a.axes && n ? a.q_pos[ax * a.q_total + doc.q0 + tok] : 0.f;
+        }
       }
-      // After a wait that ran out, only the group's barrier is still met.
-      if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(s_full + g), j & 1, abort_flag));
-      if (!ok) continue;
-      ptx::tc_fence_after();
-      uint32_t u[4][32];
+    }
+    bool ok = true;
+    auto await = [&](uint64_t* bar, int parity) {  // the same answer in all lanes
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag));
+    };
+    auto arrive = [&](uint64_t* bar) {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(bar));
+    };
+    auto meet = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + g) : "memory"); };  // the tile's eight warps
+    float* poss = reinterpret_cast<float*>(smem + L::kPos) + g * 2 * kAttnMaxAxes * kTcKeys;
+    // The positions of the keys of tile j, into the buffer of j: written before the meeting of
+    // tile j, read after it.
+    auto stage_positions = [&](int j) {
+      const int t = threadIdx.x & 255, key = j * kTcKeys + (t & 127);
+      float* put = poss + (j & 1) * kAttnMaxAxes * kTcKeys;
+      for (int ax = t >> 7; ax < a.axes; ax += 2)
+        put[ax * kTcKeys + (t & 127)] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
+    };
+    const float mul = CAP || BIAS ? 1.f : a.score_mul;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2];
+    // Caps, biases and masks 64 columns of tile j and takes the rows' largest into `top`.
+    auto prepare = [&](int j, int c, uint32_t(&x)[32], bool masked) {
+      if constexpr (CAP || BIAS) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, u[c]);
-      ptx::tmem_wait_ld();
-      float top = -INFINITY;
+        for (int e = 0; e < 32; ++e) {
+          float v = __uint_as_float(x[e]);
+          if constexpr (CAP)
+            v = attn_capped(v, a);
+          else
+            v *= a.score_mul;
+          x[e] = __float_as_uint(v);
+        }
+        if constexpr (BIAS) {
+          const float* pos = poss + (j & 1) * kAttnMaxAxes * kTcKeys + c * 64 + 2 * t4;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (CAP || BIAS) {
+          for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
+            if (ax >= a.axes) break;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float x = __uint_as_float(u[c][i]);
-            if constexpr (CAP)
-              x = attn_capped(x, a);
-            else
-              x *= a.score_mul;
-            u[c][i] = __float_as_uint(x);
-          }
-          if constexpr (BIAS) {
+            for (int k = 0; k < 8; ++k) {
+              const float2 kp = *reinterpret_cast<const float2*>(pos + ax * kTcKeys + k * 8);
 #pragma unroll
-            for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
-              if (ax >= a.axes) break;
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 kp = *reinterpret_cast<const float4*>(pos + ax * kTcKeys + c * 32 + i);
-                u[c][i] = __float_as_uint(__uint_as_float(u[c][i]) - slope[ax] * fabsf(qpos[ax] - kp.x));
-                u[c][i + 1] = __float_as_uint(__uint_as_float(u[c][i + 1]) - slope[ax] * fabsf(qpos[ax] - kp.y));
-                u[c][i + 2] = __float_as_uint(__uint_as_float(u[c][i + 2]) - slope[ax] * fabsf(qpos[ax] - kp.z));
-                u[c][i + 3] = __float_as_uint(__uint_as_float(u[c][i + 3]) - slope[ax] * fabsf(qpos[ax] - kp.w));
+              for (int e = 0; e < 2; ++e) {
+                uint32_t* y = x + 4 * k + 2 * e;
+                y[0] = __float_as_uint(__uint_as_float(y[0]) - slope[ax] * fabsf(qpos[e][ax] - kp.x));
+                y[1] = __float_as_uint(__uint_as_float(y[1]) - slope[ax] * fabsf(qpos[e][ax] - kp.y));
               }
             }
           }
         }
-        if ((j + 1) * kTcKeys > hi_low) {
-          const int lim = hi - j * kTcKeys - c * 32;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i >= lim) u[c][i] = 0xff800000u;
-        }
-        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          t0 = fmaxf(t0, __uint_as_float(u[c][i]));
-          t1 = fmaxf(t1, __uint_as_float(u[c][i + 1]));
-        }
-        top = fmaxf(top, fmaxf(t0, t1));
       }
-      const float m_new = fmaxf(m, top);
-      if (j == 0) {
-        m = m_new;
-      } else {
-        const bool grow = (m_new - m) * mul > kRescaleAt;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float shrink = grow ? exp2_fast((m - m_new) * mul) : 1.f;
-          if (grow) m = m_new;
-          l *= shrink;
-          for (int c = 0; c < a.head_dim; c += 16) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x16(to + c, o);
-            ptx::tmem_wait_ld();
-            uint32_t w[16];
+      if (masked) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-            ptx::tmem_st_32x32b_x16(to + c, w);
-          }
-        }
+        for (int e = 0; e < 32; ++e)
+          if (8 * (e >> 2) + (e & 1) >= hi[e >> 1 & 1] - (j * kTcKeys + c * 64 + 2 * t4)) x[e] = 0xff800000u;
       }
-      const float base = m == -INFINITY ? 0.f : kWeightShift - m * mul;
-      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = exp2_fast(__uint_as_float(u[c][2 * i]) * mul + base);
-          const float p1 = exp2_fast(__uint_as_float(u[c][2 * i + 1]) * mul + base);
-          sum += p0 + p1;
-          w[i] = pack2<T>(p0, p1);
-        }
-        ptx::tmem_st_32x32b_x16(ts + c * 16, w);
+        for (int k = 0; k < 8; ++k)
+          top[e] = ptx::max3_nan(top[e], __uint_as_float(x[4 * k + 2 * e]), __uint_as_float(x[4 * k + 2 * e + 1]));
+    };
+    for (int j = 0; j < n; ++j) {
+      const bool masked = (j + 1) * kTcKeys > hi_low;
+      if constexpr (BIAS) {
+        stage_positions(j);
+        meet();  // after a wait that ran out, only this is still done
       }
-      l += sum;
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_ready + g));
-    }
-    if (n > 0 && ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(s_full + g), n & 1, abort_flag));
-    if (ok) {
+      await(s_full + g, j & 1);
+      if (!ok) continue;
       ptx::tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zeros
-      T* dst = static_cast<T*>(a.out) + static_cast<long long>(doc.q0 + tok) * a.o_tok + head[g] * a.o_head;
-      for (int c = 0; c < a.head_dim; c += 16) {
+      uint32_t u[32], v[32], w[16];
+      top[0] = top[1] = -INFINITY;
+      ptx::tmem_ld_16x256b_x8(ts + 64, v);
+      ptx::tmem_wait_ld(v);
+      ptx::tmem_ld_16x256b_x8(ts, u);
+      prepare(j, 1, v, masked);
+      if constexpr (CAP || BIAS) ptx::tmem_st_16x256b_x8(ts + 64, v);  // for the second loading
+      ptx::tmem_wait_ld(u);
+      prepare(j, 0, u, masked);
+      float m_new[2];
+      bool grow = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[e] = ptx::max_nan(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+        top[e] = ptx::max_nan(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+        m_new[e] = ptx::max_nan(m[e], top[e]);
+        grow |= !((m_new[e] - m[e]) * mul <= kRescaleAt) && m_new[e] != m[e];  // NaN grows
+      }
+      if (L::kOwnP && j > 0) {  // P's columns are free, and O is at rest
+        await(o_done + g, (j - 1) & 1);
+        if (!ok) continue;
+        ptx::tc_fence_after();
+      }
+      if (j == 0) {
+        m[0] = m_new[0], m[1] = m_new[1];
+      } else if (__any_sync(0xffffffffu, grow)) {
+        float shrink[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          shrink[e] = m_new[e] == m[e] ? 1.f : exp2_fast((m[e] - m_new[e]) * mul);
+          m[e] = m_new[e];
+          l[e] *= shrink[e];
+        }
+        for (int c = 0; c < a.head_dim; c += 16) {
+          uint32_t o[8];
+          ptx::tmem_ld_16x256b_x2(to + c, o);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink[e >> 1 & 1]);
+          ptx::tmem_st_16x256b_x2(to + c, o);
+        }
+      }
+      uint64_t base[2], sum[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // A row that has seen nothing yet weighs nothing; an infinite score makes a NaN, as the
+        // formula does.
+        const float shift = m[e] == -INFINITY ? 0.f : kWeightShift - m[e] * mul;
+        const float b = m[e] == INFINITY ? NAN : shift;
+        base[e] = ptx::pack_f2(b, b);
+      }
+      const uint64_t mul2 = ptx::pack_f2(mul, mul);
+      if constexpr (CAP || BIAS) ptx::tmem_wait_st();
+      ptx::tmem_ld_16x256b_x8(ts + 64, v);
+      weights32<T>(u, mul2, base, w, sum);
+      ptx::tmem_st_16x128b_x8(tp, w);
+      ptx::tmem_wait_ld(v);
+      if constexpr (L::kOwnP) arrive(s_free + g);
+      if (!CAP && !BIAS && masked) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (8 * (e >> 2) + (e & 1) >= hi[e >> 1 & 1] - (j * kTcKeys + 64 + 2 * t4)) v[e] = 0xff800000u;
+      }
+      weights32<T>(v, mul2, base, w, sum);
+      ptx::tmem_st_16x128b_x8(tp + 32, w);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 s2 = ptx::unpack_f2(sum[e]);
+        l[e] += s2.x + s2.y;
+      }
+      ptx::tmem_wait_st();
+      arrive(p_ready + g);
+    }
+    if (n > 0) {
+      if constexpr (L::kOwnP)
+        await(o_done + g, (n - 1) & 1);
+      else
+        await(s_full + g, n & 1);
+    }
+    float* sums = reinterpret_cast<float*>(smem + L::kSums) + g * kTcRows;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if (t4 == 0) sums[row16 + (lane >> 2) + 8 * e] = l[e];
+    }
+    meet();
+    if (ok) {  // two warps to 32 rows, a thread to a row: every other 16 columns each
+      ptx::tc_fence_after();
+      const int r = (warp & 3) * 32 + lane;
+      const float sum = sums[r];
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zeros
+      T* dst = static_cast<T*>(a.out) + static_cast<long long>(doc.q0 + tok0[g] + r) * a.o_tok + head[g] * a.o_head;
+      const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + L::kColO + g * L::kCols;
+      for (int c = (warp >> 2 & 1) * 16; c < a.head_dim; c += 32) {
         uint32_t o[32];
         if (n > 0) {
-          ptx::tmem_ld_32x32b_x16(to + c, o);
+          ptx::tmem_ld_32x32b_x16(from + c, o);
           ptx::tmem_wait_ld();
         }
-        if (!mine) continue;
-        uint4 w[2];
-        uint32_t* p = reinterpret_cast<uint32_t*>(w);
+        if (r >= ntok[g]) continue;
+        uint4 q[2];
+        uint32_t* p = reinterpret_cast<uint32_t*>(q);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           p[i] = n > 0 ? pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
-        *reinterpret_cast<uint4*>(dst + c) = w[0];
-        if (c + 8 < a.head_dim) *reinterpret_cast<uint4*>(dst + c + 8) = w[1];
+        *reinterpret_cast<uint4*>(dst + c) = q[0];
+        if (c + 8 < a.head_dim) *reinterpret_cast<uint4*>(dst + c + 8) = q[1];
       }
     }
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (warp == 9) ptx::tmem_dealloc(tmem, 512);
+  if (warp == kProductWarp) ptx::tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag) atomicOr(a.status, 1u);
 }
 
