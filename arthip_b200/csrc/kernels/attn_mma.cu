@@ -19,7 +19,7 @@
 // joined at the end. Either may share its keys out over a cluster of CTAs, whose partial
 // results are joined through distributed shared memory, so no workspace is needed and the
 // order of the sums is fixed.
-#include "attn_common.cuh"
+#include "token_common.cuh"
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

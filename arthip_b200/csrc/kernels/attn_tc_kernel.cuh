@@ -29,7 +29,7 @@
 // Every wait is bounded; one that runs out ends the CTA and sets the status word.
 #pragma once
 
-#include "attn_common.cuh"
+#include "token_common.cuh"
 #include "ptx.cuh"
 #include "tokens.h"
 

@@ -1,4 +1,4 @@
-// What the two attention kernels share: the capped score and the launch attributes.
+// What the token kernels share: the capped score of attention, and launch attributes.
 #pragma once
 
 #include "tokens.h"

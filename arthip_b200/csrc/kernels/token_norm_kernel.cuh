@@ -1,0 +1,617 @@
+// The norms around a block, its gate and its residual scale in one pass over the rows:
+//
+//   b    = post(y) * A[c] (+ B[c])        post: none, RMS or layer norm; A holds the norm's
+//                                         weight times layer scale times residual scale
+//   out  = x + act(gate) * b
+//   norm = pre(out) * w[c] (+ wb[c]),     then * (1 + mscale) + mshift
+//
+// Everything is fp32 in registers from load to store. Both norms read unrounded values: the
+// pre-norm's statistics are those of the fp32 sum, not of the fp16 / bf16 row written out.
+// A layer norm takes its variance from the centred values in a second sweep over the
+// registers, so a large mean costs no digits.
+//
+// Bound: HBM, 8 bytes per element (y, x in; out, norm out), 10 with a per-token gate. Two
+// kernels: rows of whole vectors of 16, 8 or 4 bytes, and rows of any width, stride or
+// alignment, which pass through shared memory in 16-byte pieces all the same (loaded element by
+// element, 91 channels ran at 9% of the copy rate; this way at 40%).
+#pragma once
+
+#include "token_common.cuh"
+#include "tokens.h"
+
+#include <algorithm>
+#include <atomic>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace ah {
+namespace token_norm {
+
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ void from_f(float v, __half* o) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f2(float a, float b, __half2* o) { *o = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void from_f2(float a, float b, __nv_bfloat162* o) { *o = __floats2bfloat162_rn(a, b); }
+
+template <typename T>
+struct Two;
+template <>
+struct Two<__half> {
+  using type = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T e[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& u, float (&f)[V]) {
+  if constexpr (V % 2 == 0) {
+    const auto* p = reinterpret_cast<const typename Two<T>::type*>(&u);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 t = to_f2(p[i]);
+      f[2 * i] = t.x, f[2 * i + 1] = t.y;
+    }
+  } else {
+    f[0] = to_f(u.e[0]);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+  Vec<T, V> u;
+  if constexpr (V % 2 == 0) {
+    auto* q = reinterpret_cast<typename Two<T>::type*>(&u);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) from_f2(f[2 * i], f[2 * i + 1], q + i);
+  } else {
+    from_f(f[0], &u.e[0]);
+  }
+  *reinterpret_cast<Vec<T, V>*>(p) = u;
+}
+
+// V floats of a weight array, 16 bytes at a time where V allows, or `fill` without one.
+template <int V>
+__device__ __forceinline__ void load_weight(const float* p, int c, float fill, float (&f)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = fill;
+    return;
+  }
+  p += c;
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+      f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = __ldg(p + i);
+  }
+}
+
+__device__ __forceinline__ float gate_act(float g, int act) {
+  if (act == kGateTanh) return tanhf(g);
+  if (act == kGateLinear) return g;
+  const float s = __fdividef(1.f, 1.f + __expf(-g));  // a few fp32 ulp, 0 for very negative g
+  return act == kGateSilu ? (s == 0.f ? s : g * s) : s;
+}
+
+// Sum over the L lanes of a warp that hold a row, or (L = 0) over `warps` whole warps that meet
+// at the named barrier `bar` and leave their sums in `red`.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* red, int warps, int bar) {
+#pragma unroll
+  for (int o = (L ? L : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (L == 0) {
+    const int w = (threadIdx.x >> 5) % warps;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");  // the last sum has been read
+    if ((threadIdx.x & 31) == 0) red[w] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
+    v = 0.f;
+    for (int i = 0; i < warps; ++i) v += red[i];
+  }
+  return v;
+}
+
+// Of a lane's share of a row, E values of which in(e) lie in the row (the others are zeros):
+// v -> (v - mean) * rstd as v * mul + add. Four running sums, so that additions overlap.
+template <int L, int E, typename In>
+__device__ __forceinline__ void statistics(const float (&f)[E], In in, int kind, float eps, float inv_c, float* red,
+                                           int warps, int bar, float* mul, float* add) {
+  *mul = 1.f, *add = 0.f;
+  if (kind == kNormNone) return;
+  float mean = 0.f;
+  if (kind == kNormLayer) {
+    float s[4] = {};
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e & 3] += f[e];
+    mean = row_sum<L>((s[0] + s[1]) + (s[2] + s[3]), red, warps, bar) * inv_c;
+  }
+  float s[4] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float d = f[e] - mean;
+    if (in(e)) s[e & 3] += d * d;
+  }
+  *mul = rsqrtf(row_sum<L>((s[0] + s[1]) + (s[2] + s[3]), red, warps, bar) * inv_c + eps);
+  *add = -mean * *mul;
+}
+
+// ---------------------------------------------------------------------------
+// Rows of vectors of 16, 8 or 4 bytes
+// ---------------------------------------------------------------------------
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int V, int E>
+__device__ __forceinline__ float (&part(float (&f)[E], int n))[V] {
+  return *reinterpret_cast<float(*)[V]>(f + n * V);
+}
+
+// A row is held by L lanes of a warp, or (L = 0) by `row_warps` whole warps, N vectors per
+// lane: vector n of lane l starts at channel (n * lanes + l) * kV. Each group of lanes walks
+// over rows. The next row's loads are issued before this row is worked on, so that memory is not
+// idle behind the sums that a row waits for, as asynchronous copies into the lane's own places
+// in shared memory: no thread waits for another, and they cost no registers (held in registers
+// instead, 1280 channels ran at 60% of the copy rate, this way at 77%).
+template <typename T, int kV, int L, int N, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row_warps) {
+  extern __shared__ __align__(16) uint8_t smem[];  // [2 rows][x, y][N][threads] vectors
+  __shared__ float red_all[32];
+  const int lanes = L ? L : row_warps * 32;
+  const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+  float* red = red_all + (L ? 0 : group * row_warps);
+  const int bar = 1 + (L ? 0 : group);
+  const int groups = blockDim.x / lanes;
+  const long long step = static_cast<long long>(gridDim.x) * groups;
+  const float inv_c = 1.f / static_cast<float>(a.C);
+  const T* x = static_cast<const T*>(a.x);
+  const T* y = static_cast<const T*>(a.y);
+  const T* gate = static_cast<const T*>(a.gate);
+
+  bool in[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) in[n] = (n * lanes + lane) * kV < a.C;
+  auto held = [&](int e) { return in[e / kV]; };
+  float ka[kV], kw[kV];
+  if constexpr (N == 1) {
+    load_weight<kV>(a.a, in[0] ? lane * kV : 0, 1.f, ka);
+    load_weight<kV>(a.w, in[0] ? lane * kV : 0, 1.f, kw);
+  }
+
+  auto place = [&](int buf, int stream, int n) {
+    return reinterpret_cast<Vec<T, kV>*>(smem) + ((buf * 2 + stream) * N + n) * THREADS + threadIdx.x;
+  };
+  auto fetch = [&](long long row, int buf) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = (n * lanes + lane) * kV;
+      if (!in[n]) continue;
+      copy_async<kV * 2>(place(buf, 0, n), x + row * a.xs + c);
+      if (y) copy_async<kV * 2>(place(buf, 1, n), y + row * a.ys + c);
+    }
+  };
+  // All lanes of a warp take as many steps as its first group, for the shuffles: a group
+  // whose row lies past the end works on an old row (or zeros) and stores nothing.
+  long long row = static_cast<long long>(blockIdx.x) * groups + group;
+  long long row0 = L ? static_cast<long long>(blockIdx.x) * groups + (threadIdx.x & ~31) / lanes : row;
+  if (row < a.rows) fetch(row, 0);
+  copies_commit();
+  for (int buf = 0; row0 < a.rows; row += step, row0 += step, buf ^= 1) {
+    const bool live = row < a.rows;
+    if (row + step < a.rows) fetch(row + step, buf ^ 1);
+    copies_commit();
+    copies_wait<1>();
+    float r[N * kV], mul, add;  // y (without one, x), then the sum
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float(&f)[kV] = part<kV>(r, n);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) f[i] = 0.f;
+      if (in[n]) unpack<T, kV>(*place(buf, y ? 1 : 0, n), f);
+    }
+    if (y) {
+      const T* grow = nullptr;
+      if (gate && live) grow = gate + (a.rows_per_gate == 1 ? row : row / a.rows_per_gate) * a.gs;
+      statistics<L, N * kV>(r, held, a.post, a.post_eps, inv_c, red, row_warps, bar, &mul, &add);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int c = (n * lanes + lane) * kV;
+        if (!in[n]) continue;
+        float(&f)[kV] = part<kV>(r, n);
+        float xf[kV];
+        unpack<T, kV>(*place(buf, 0, n), xf);
+        if constexpr (N > 1) load_weight<kV>(a.a, c, 1.f, ka);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) f[i] = (f[i] * mul + add) * ka[i];
+        if (a.b) {
+          float kb[kV];
+          load_weight<kV>(a.b, c, 0.f, kb);
+#pragma unroll
+          for (int i = 0; i < kV; ++i) f[i] += kb[i];
+        }
+        if (grow) {
+          float g[kV];
+          unpack<T, kV>(load<T, kV>(grow + c), g);
+          if (a.act != kGateLinear) {
+#pragma unroll
+            for (int i = 0; i < kV; ++i) g[i] = gate_act(g[i], a.act);
+          }
+#pragma unroll
+          for (int i = 0; i < kV; ++i) f[i] *= g[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i) f[i] += xf[i];
+      }
+    }
+    if (a.out && live) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (in[n]) store<T, kV>(static_cast<T*>(a.out) + row * a.os + (n * lanes + lane) * kV, part<kV>(r, n));
+    }
+    if (!a.norm) continue;
+    statistics<L, N * kV>(r, held, a.pre, a.pre_eps, inv_c, red, row_warps, bar, &mul, &add);
+    if (!live) continue;
+    const long long mrow = (a.mscale || a.mshift) ? row / a.rows_per_mod * a.ms : 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = (n * lanes + lane) * kV;
+      if (!in[n]) continue;
+      float(&f)[kV] = part<kV>(r, n);
+      if constexpr (N > 1) load_weight<kV>(a.w, c, 1.f, kw);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) f[i] = (f[i] * mul + add) * kw[i];
+      if (a.wb) {
+        float kb[kV];
+        load_weight<kV>(a.wb, c, 0.f, kb);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) f[i] += kb[i];
+      }
+      float m[kV];
+      if (a.mscale) {
+        unpack<T, kV>(load<T, kV>(static_cast<const T*>(a.mscale) + mrow + c), m);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) f[i] += f[i] * m[i];
+      }
+      if (a.mshift) {
+        unpack<T, kV>(load<T, kV>(static_cast<const T*>(a.mshift) + mrow + c), m);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) f[i] += m[i];
+      }
+      store<T, kV>(static_cast<T*>(a.norm) + row * a.ns + c, f);
+    }
+  }
+}
+
+// As many blocks as fit at once (the same on every sm_100 GPU), each walking over its work.
+template <typename F>
+cudaError_t resident_blocks(F fn, int threads, size_t smem, int num_sms, std::atomic<int>* known, long long* blocks) {
+  int per_sm = known->load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, smem);
+    if (e != cudaSuccess) return e;
+    known->store(per_sm, std::memory_order_relaxed);
+  }
+  *blocks = static_cast<long long>(num_sms) * per_sm;
+  return cudaSuccess;
+}
+
+template <typename T, int kV, int L, int N, int THREADS>
+cudaError_t launch(const NormArgs& a, int row_warps, int num_sms, cudaStream_t s) {
+  auto fn = norm_kernel<T, kV, L, N, THREADS>;
+  static std::atomic<int> known[33];  // by row_warps
+  const int groups = THREADS / (L ? L : row_warps * 32);
+  long long most;
+  constexpr int kSmem = 4 * N * THREADS * kV * 2;
+  static AttrOnce once;
+  cudaError_t e = once.set(reinterpret_cast<const void*>(fn), kSmem);
+  if (e == cudaSuccess) e = resident_blocks(fn, THREADS, kSmem, num_sms, known + row_warps, &most);
+  if (e != cudaSuccess) return e;
+  const long long blocks = std::min<long long>((a.rows + groups - 1) / groups, most);
+  fn<<<static_cast<unsigned>(blocks), THREADS, kSmem, s>>>(a, row_warps);
+  return cudaGetLastError();
+}
+
+// Two or three vectors a lane where the width allows, so that a row's fixed work is shared by
+// few lanes (64 channels on eight lanes of one vector: 80% of the copy rate, on four of two:
+// 93%); a warp to a row while that holds it, as sums across warps cost two barriers each.
+template <typename T, int V>
+cudaError_t by_width(const NormArgs& a, int num_sms, cudaStream_t s) {
+  const int n = a.C / V;  // vectors in a row
+  if (n <= 4) return launch<T, V, 4, 1, 256>(a, 1, num_sms, s);
+  if (n <= 8) return launch<T, V, 4, 2, 256>(a, 1, num_sms, s);
+  if (n <= 12) return launch<T, V, 4, 3, 256>(a, 1, num_sms, s);
+  if (n <= 16) return launch<T, V, 8, 2, 256>(a, 1, num_sms, s);
+  if (n <= 24) return launch<T, V, 8, 3, 256>(a, 1, num_sms, s);
+  if (n <= 32) return launch<T, V, 16, 2, 256>(a, 1, num_sms, s);
+  if (n <= 48) return launch<T, V, 16, 3, 256>(a, 1, num_sms, s);
+  if (n <= 64) return launch<T, V, 32, 2, 256>(a, 1, num_sms, s);
+  if (n <= 96) return launch<T, V, 32, 3, 128>(a, 1, num_sms, s);
+  if (n <= 128) return launch<T, V, 32, 4, 128>(a, 1, num_sms, s);
+  if (n <= 160) return launch<T, V, 32, 5, 128>(a, 1, num_sms, s);
+  if (n <= 192) return launch<T, V, 32, 6, 128>(a, 1, num_sms, s);
+  if (n <= 256) return launch<T, V, 0, 4, 128>(a, 2, num_sms, s);
+  if (n <= 384) return launch<T, V, 0, 6, 128>(a, 2, num_sms, s);
+  if (n <= 512) return launch<T, V, 0, 4, 128>(a, 4, num_sms, s);
+  if (n <= 768) return launch<T, V, 0, 6, 128>(a, 4, num_sms, s);
+  if (n <= 1024) return launch<T, V, 0, 4, 256>(a, 8, num_sms, s);
+  // n is at most 8192 / V
+  if constexpr (V < 8)
+    if (n <= 2048) return launch<T, V, 0, 8, 256>(a, 8, num_sms, s);
+  if constexpr (V == 2) return launch<T, V, 0, 16, 256>(a, 8, num_sms, s);
+  return cudaErrorInvalidValue;
+}
+
+// ---------------------------------------------------------------------------
+// Any rows, through shared memory
+// ---------------------------------------------------------------------------
+// A group of GROUP threads (a warp, or the block for wide rows) takes a tile of some rows: their
+// elements come into shared memory by asynchronous 16-byte copies, one tile ahead, the elements
+// before the first and behind the last 16-byte boundary one by one; the results leave the same
+// way. LANES lanes share a row (a warp has 32 / LANES at once), element e being lane e % LANES'.
+// A lane's N channels are the same in every row, and their weights stay in registers. N is even
+// and at most one more than a lane needs, so that only its last two elements are ever in
+// question: with a test for each (N in steps of 4 and 8), 90 channels took 85 instructions an
+// element and ran at 34% of the copy rate.
+template <int GROUP>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (GROUP == 32)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / GROUP), "n"(GROUP) : "memory");
+}
+
+// Elements [0, n) of `src` to where `dst` + (src % 16 bytes) starts. Waits for nothing.
+template <typename T, int GROUP>
+__device__ __forceinline__ void copy_in(uint8_t* dst, const T* src, int n, int t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(src);
+  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
+  T* d = reinterpret_cast<T*>(dst + at % 16);
+  if (t < head) d[t] = src[t];
+  for (int i = t; i < body; i += GROUP)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(d + head + 8 * i))),
+                 "l"(src + head + 8 * i)
+                 : "memory");
+  const int tail = head + body * 8 + t;
+  if (tail < n) d[tail] = src[tail];
+}
+
+// The way back: elements [0, n) from `src` + (dst % 16 bytes).
+template <typename T, int GROUP>
+__device__ __forceinline__ void copy_out(T* dst, const uint8_t* src, int n, int t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
+  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
+  const T* from = reinterpret_cast<const T*>(src + at % 16);
+  if (t < head) dst[t] = from[t];
+  for (int i = t; i < body; i += GROUP)
+    *reinterpret_cast<uint4*>(dst + head + 8 * i) = *reinterpret_cast<const uint4*>(from + head + 8 * i);
+  const int tail = head + body * 8 + t;
+  if (tail < n) dst[tail] = from[tail];
+}
+
+struct Tiles {
+  int rows = 1;         // of a tile
+  int slot = 0;         // bytes of one stream's tile in shared memory
+  int streams = 2;      // x, y and a per-token gate
+  long long count = 0;
+};
+
+template <typename T, int GROUP, int LANES, int N>
+__global__ void __launch_bounds__(256, N <= 8 ? 3 : (N <= 16 ? 2 : 1)) norm_staged_kernel(const NormArgs a, const Tiles tiles) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red_all[8];
+  constexpr int L = GROUP == 32 ? LANES : 0;  // LANES is GROUP when that is more than a warp
+  constexpr int kRows = GROUP / LANES;        // at once
+  const int t = threadIdx.x % GROUP, lane = t % LANES, group = threadIdx.x / GROUP;
+  float* red = red_all + (L ? 0 : group * (GROUP / 32));
+  const int bar = 1 + group;
+  const int groups = 256 / GROUP;
+  const int slots = 2 * tiles.streams + 2;
+  uint8_t* base = smem + static_cast<size_t>(group) * slots * tiles.slot;
+  uint8_t* s_out = base + 2 * tiles.streams * tiles.slot;
+  uint8_t* s_norm = s_out + tiles.slot;
+  const float inv_c = 1.f / static_cast<float>(a.C);
+  const T* x = static_cast<const T*>(a.x);
+  const T* y = static_cast<const T*>(a.y);
+  const T* gate = static_cast<const T*>(a.gate);
+  const bool row_gate = gate && a.rows_per_gate == 1;
+  const bool in0 = (N - 2) * LANES + lane < a.C, in1 = (N - 1) * LANES + lane < a.C;
+  auto in = [&](int k) { return k < N - 2 || (k == N - 2 ? in0 : in1); };
+  float ka[N], kw[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    ka[k] = a.a && in(k) ? a.a[lane + k * LANES] : 1.f;
+    kw[k] = a.w && in(k) ? a.w[lane + k * LANES] : 1.f;
+  }
+  auto offset = [](const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16); };
+  auto rows_of = [&](long long tile) {
+    return static_cast<int>(min(static_cast<long long>(tiles.rows), a.rows - tile * tiles.rows));
+  };
+  auto fetch = [&](long long tile, int buf) {
+    uint8_t* to = base + buf * tiles.streams * tiles.slot;
+    const long long row = tile * tiles.rows;
+    const int n = (rows_of(tile) - 1) * a.C + a.C;
+    copy_in<T, GROUP>(to, x + row * a.xs, n, t);
+    if (y) copy_in<T, GROUP>(to + tiles.slot, y + row * a.ys, n, t);
+    if (row_gate) copy_in<T, GROUP>(to + 2 * tiles.slot, gate + row * a.gs, n, t);
+  };
+  const long long step = static_cast<long long>(gridDim.x) * groups;
+  long long tile = static_cast<long long>(blockIdx.x) * groups + group;
+  if (tile < tiles.count) fetch(tile, 0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  for (int buf = 0; tile < tiles.count; tile += step, buf ^= 1) {
+    if (tile + step < tiles.count) fetch(tile + step, buf ^ 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    group_sync<GROUP>();
+    const uint8_t* from = base + buf * tiles.streams * tiles.slot;
+    const long long row0 = tile * tiles.rows;
+    const int n_rows = rows_of(tile);
+    const T* sx = reinterpret_cast<const T*>(from + offset(x + row0 * a.xs));
+    const T* sy = reinterpret_cast<const T*>(from + tiles.slot + offset(y + row0 * a.ys));
+    const T* sg = reinterpret_cast<const T*>(from + 2 * tiles.slot + offset(gate + row0 * a.gs));
+    T* out = static_cast<T*>(a.out) + row0 * a.os;
+    T* norm = static_cast<T*>(a.norm) + row0 * a.ns;
+    T* so = reinterpret_cast<T*>(s_out + offset(out));
+    T* sn = reinterpret_cast<T*>(s_norm + offset(norm));
+    for (int i0 = 0; i0 < n_rows; i0 += kRows) {  // past the last row its lanes repeat it
+      const int i = min(i0 + t / LANES, n_rows - 1);
+      const bool mine = i0 + t / LANES < n_rows;
+      const long long row = row0 + i;
+      const T* xi = sx + i * a.C + lane;
+      float r[N], mul, add;
+#pragma unroll
+      for (int k = 0; k < N; ++k) r[k] = in(k) ? to_f(xi[k * LANES]) : 0.f;
+      if (y) {
+        const T* yi = sy + i * a.C + lane;
+        float f[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = in(k) ? to_f(yi[k * LANES]) : 0.f;
+        statistics<L, N>(f, in, a.post, a.post_eps, inv_c, red, GROUP / 32, bar, &mul, &add);
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = (f[k] * mul + add) * ka[k];
+        if (a.b) {
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (in(k)) f[k] += __ldg(a.b + lane + k * LANES);
+        }
+        if (gate) {
+          const T* gi = (row_gate ? sg + i * a.C : gate + row / a.rows_per_gate * a.gs) + lane;
+          float g[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) g[k] = in(k) ? to_f(gi[k * LANES]) : 0.f;
+          if (a.act != kGateLinear) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) g[k] = gate_act(g[k], a.act);
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k) f[k] *= g[k];
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) r[k] = in(k) ? r[k] + f[k] : 0.f;
+      }
+      if (a.out && mine) {
+        T* oi = so + i * a.C + lane;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (in(k)) from_f(r[k], oi + k * LANES);
+      }
+      if (!a.norm) continue;
+      statistics<L, N>(r, in, a.pre, a.pre_eps, inv_c, red, GROUP / 32, bar, &mul, &add);
+#pragma unroll
+      for (int k = 0; k < N; ++k) r[k] = (r[k] * mul + add) * kw[k];
+      if (a.wb) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (in(k)) r[k] += __ldg(a.wb + lane + k * LANES);
+      }
+      if (a.mscale || a.mshift) {
+        const long long mrow = row / a.rows_per_mod * a.ms + lane;
+        const T* scale = static_cast<const T*>(a.mscale) + mrow;
+        const T* shift = static_cast<const T*>(a.mshift) + mrow;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          if (!in(k)) continue;
+          if (a.mscale) r[k] += r[k] * to_f(scale[k * LANES]);
+          if (a.mshift) r[k] += to_f(shift[k * LANES]);
+        }
+      }
+      if (!mine) continue;
+      T* ni = sn + i * a.C + lane;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (in(k)) from_f(r[k], ni + k * LANES);
+    }
+    group_sync<GROUP>();
+    if (a.out) copy_out<T, GROUP>(out, s_out, n_rows * a.C, t);
+    if (a.norm) copy_out<T, GROUP>(norm, s_norm, n_rows * a.C, t);
+    group_sync<GROUP>();  // the results have left, and the inputs may be written over
+  }
+}
+
+template <typename T, int GROUP, int LANES, int N>
+cudaError_t launch_staged(const NormArgs& a, int num_sms, cudaStream_t s) {
+  auto fn = norm_staged_kernel<T, GROUP, LANES, N>;
+  Tiles tiles;
+  auto packed = [&](const void* p, long long stride) { return !p || stride == a.C; };
+  const bool row_gate = a.gate && a.rows_per_gate == 1;
+  tiles.streams = row_gate ? 3 : 2;
+  if (packed(a.x, a.xs) && packed(a.y, a.ys) && packed(a.out, a.os) && packed(a.norm, a.ns) &&
+      (!row_gate || a.gs == a.C)) {
+    // About 2 KB of each stream, but enough tiles for every warp: rows of other pitch go one by one.
+    constexpr int kRows = GROUP / LANES;
+    const long long fair = std::max<long long>(kRows, a.rows / (num_sms * 16LL) / kRows * kRows);
+    tiles.rows = static_cast<int>(std::clamp<long long>(1024 / a.C / kRows * kRows, kRows, fair));
+  }
+  tiles.slot = (tiles.rows * a.C * 2 + 15) / 16 * 16 + 16;
+  tiles.count = (a.rows + tiles.rows - 1) / tiles.rows;
+  const int groups = 256 / GROUP;
+  const size_t smem = static_cast<size_t>(groups) * (2 * tiles.streams + 2) * tiles.slot;
+  static AttrOnce once;
+  cudaError_t e = once.set(reinterpret_cast<const void*>(fn), 200 * 1024);
+  if (e != cudaSuccess) return e;
+  const int per_sm = static_cast<int>(std::clamp<size_t>(220 * 1024 / (smem + 1024), 1, 8));
+  const long long blocks = std::min<long long>((tiles.count + groups - 1) / groups, static_cast<long long>(num_sms) * per_sm);
+  fn<<<static_cast<unsigned>(blocks), 256, smem, s>>>(a, tiles);
+  return cudaGetLastError();
+}
+
+// The launch with the N that C needs of [LO, HI] (even numbers), LANES lanes a row.
+template <typename T, int GROUP, int LANES, int LO, int HI>
+cudaError_t by_count(const NormArgs& a, int num_sms, cudaStream_t s) {
+  if constexpr (LO < HI)
+    if (a.C > LO * LANES) return by_count<T, GROUP, LANES, LO + 2, HI>(a, num_sms, s);
+  return launch_staged<T, GROUP, LANES, LO>(a, num_sms, s);
+}
+
+// 5 to 16 elements a lane: a row's fixed work (the sums across lanes, the choices) is shared by
+// as many rows at once as that leaves lanes for.
+template <typename T>
+cudaError_t by_elements(const NormArgs& a, int num_sms, cudaStream_t s) {
+  if (a.C <= 32) return by_count<T, 32, 4, 2, 8>(a, num_sms, s);
+  if (a.C <= 64) return by_count<T, 32, 8, 6, 8>(a, num_sms, s);
+  if (a.C <= 128) return by_count<T, 32, 16, 6, 8>(a, num_sms, s);
+  if (a.C <= 512) return by_count<T, 32, 32, 6, 16>(a, num_sms, s);
+  if (a.C <= 1024) return by_count<T, 64, 64, 10, 16>(a, num_sms, s);
+  if (a.C <= 2048) return by_count<T, 128, 128, 10, 16>(a, num_sms, s);
+  if (a.C <= 4096) return by_count<T, 256, 256, 10, 16>(a, num_sms, s);
+  return by_count<T, 256, 256, 20, 32>(a, num_sms, s);
+}
+
+// One translation unit each (token_norm_*.cu): rows of vectors (of `vec` elements), any rows.
+cudaError_t vectors_f16(const NormArgs& a, int vec, int num_sms, cudaStream_t s);
+cudaError_t vectors_bf16(const NormArgs& a, int vec, int num_sms, cudaStream_t s);
+cudaError_t elements_f16(const NormArgs& a, int num_sms, cudaStream_t s);
+cudaError_t elements_bf16(const NormArgs& a, int num_sms, cudaStream_t s);
+
+}  // namespace token_norm
+}  // namespace ah
