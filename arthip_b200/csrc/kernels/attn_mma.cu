@@ -14,12 +14,16 @@
 // Keys and values beyond a document's keys in use are filled with zeros as they are staged,
 // whatever the memory holds, so a NaN there cannot reach a sum through a weight of zero.
 //
-// Two forms: 64 rows, each warp 16 of them with all keys of a tile; or 16 rows, for a few
+// Three forms: 64 rows, each warp 16 of them with all keys of a tile; or 16 rows, for a few
 // query tokens, where each warp takes 16 of a tile's 64 keys and the four partial results are
-// joined at the end. Either may share its keys out over a cluster of CTAs, whose partial
-// results are joined through distributed shared memory, so no workspace is needed and the
-// order of the sums is fixed.
+// joined at the end; each of them with its keys shared out over a cluster of CTAs, whose
+// partial results are joined through distributed shared memory, so that no workspace is needed
+// and the order of the sums is fixed; and 64 rows with all their keys in one CTA, which takes
+// some key heads one after another, the next one's loads under way, and writes its rows itself.
 #include "token_common.cuh"
+#include "tokens.h"
+
+#include <algorithm>
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -33,6 +37,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kStages = 3;
+constexpr float kWeightShift = 6.f;  // weights are 2^(x - max + 6): a wider range above fp16's smallest
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -91,21 +96,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-template <int DP, bool FEW>
+enum Form : int { kFew = 0, kWideShared = 1, kWideAlone = 2 };
+
+template <int DP, int FORM>
 struct Layout {
+  static constexpr bool FEW = FORM == kFew;
   static constexpr int kRow = DP * 2 + 16;  // bytes of a staged row: 16 more than it holds, for the banks
   static constexpr int kTile = kMmaKeys * kRow;
-  static constexpr int kStage = 2 * kTile + kAttnMaxAxes * kMmaKeys * 4;
-  static constexpr int kQ = (FEW ? kMmaRowsFew : kMmaRowsWide) * kRow;
-  static constexpr int kBytes = kQ + kStages * kStage;
+  static constexpr int kPos = 2 * kTile;  // in a stage: keys, values, key positions, queries
+  static constexpr int kStageQ = kPos + kAttnMaxAxes * kMmaKeys * 4;
+  static constexpr int kStage = kStageQ + (FORM == kWideAlone ? kMmaRowsWide * kRow : 0);
+  static constexpr int kQ = FORM == kWideAlone ? 0 : (FEW ? kMmaRowsFew : kMmaRowsWide) * kRow;
+  static constexpr int bytes(int stages) { return kQ + stages * kStage; }
   // partial results, in the place of the stages
   static constexpr int kPartRow = DP + 4;  // floats
   static_assert(kStages * kStage >= 4 * 16 * kPartRow * 4 + 4 * 16 * 2 * 4, "partial results do not fit");
 };
 
-template <typename T, int DP, bool FEW>
-__global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constant__ AttnArgs a) {
-  using L = Layout<DP, FEW>;
+template <typename T, int DP, int FORM>
+__global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 : 1)
+    attn_mma_kernel(const __grid_constant__ AttnArgs a) {
+  using L = Layout<DP, FORM>;
+  constexpr bool FEW = L::FEW;
   constexpr int kRows = FEW ? kMmaRowsFew : kMmaRowsWide;
   constexpr int kWarpKeys = FEW ? kMmaKeys / 4 : kMmaKeys;  // of a tile
   constexpr int kNT = kWarpKeys / 8;
@@ -114,14 +126,15 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
   uint8_t* sQ = smem;
   uint8_t* sStage = smem + L::kQ;
   cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
+  const int ranks = FORM == kWideAlone ? 1 : static_cast<int>(cluster.num_blocks());
+  const int rank = FORM == kWideAlone ? 0 : static_cast<int>(cluster.block_rank());
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const AttnItem item = a.items[blockIdx.x / ranks];
   const AttnDoc doc = a.docs[item.doc];
-  const int kvh = blockIdx.y;
+  const int kvh0 = blockIdx.y * (FORM == kWideAlone ? a.heads_per_block : 1);
+  const int heads = FORM == kWideAlone ? min(a.heads_per_block, a.kv_heads - kvh0) : 1;  // one after another
   int klen = doc.nk;
   if (a.k_lens) klen = min(max(a.k_lens[item.doc], 0), doc.nk);
   const int rows = min(kRows, doc.nq * a.group - item.row0);
@@ -138,35 +151,12 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
   const int tile0 = static_cast<int>(static_cast<long long>(tiles) * rank / ranks);
   const int tile1 = static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / ranks);
 
-  const T* kbase = static_cast<const T*>(a.k) + doc.k0 * a.k_tok + kvh * a.k_head;
-  const T* vbase = static_cast<const T*>(a.v) + doc.k0 * a.v_tok + kvh * a.v_head;
+  const int tiles_here = tile1 - tile0, steps = tiles_here * heads;
   const int chunks = a.head_dim / 8;
 
-  auto load_tile = [&](int tile) {
-    uint8_t* st = sStage + (tile - tile0) % kStages * L::kStage;
-    const uint32_t sk = static_cast<uint32_t>(__cvta_generic_to_shared(st));
-    constexpr int kC = DP / 8;
-    for (int i = threadIdx.x; i < kMmaKeys * kC; i += kThreads) {
-      const int r = i / kC, c = i % kC;
-      const int key = tile * kMmaKeys + r;
-      const bool take = key < klen && c < chunks;
-      const long long kk = take ? key : 0;
-      const int cc = take ? c * 8 : 0;
-      cp_async16(sk + r * L::kRow + c * 16, kbase + kk * a.k_tok + cc, take);
-      cp_async16(sk + L::kTile + r * L::kRow + c * 16, vbase + kk * a.v_tok + cc, take);
-    }
-    if (a.axes) {
-      float* sp = reinterpret_cast<float*>(st + 2 * L::kTile);
-      for (int i = threadIdx.x; i < a.axes * kMmaKeys; i += kThreads) {
-        const int ax = i / kMmaKeys, key = tile * kMmaKeys + i % kMmaKeys;
-        sp[i] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
-      }
-    }
-  };
-
-  // Queries of the block, rows past its end as zeros.
-  {
-    const uint32_t sq = static_cast<uint32_t>(__cvta_generic_to_shared(sQ));
+  // Queries of the block for one key head, rows past its end as zeros.
+  auto load_queries = [&](uint8_t* to, int kvh) {
+    const uint32_t sq = static_cast<uint32_t>(__cvta_generic_to_shared(to));
     constexpr int kC = DP / 8;
     for (int i = threadIdx.x; i < kRows * kC; i += kThreads) {
       const int r = i / kC, c = i % kC;
@@ -176,10 +166,55 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
                      (kvh * a.group + row % a.group) * a.q_head + (take ? c * 8 : 0);
       cp_async16(sq + r * L::kRow + c * 16, src, take);
     }
-  }
+  };
+  // Step s is tile tile0 + s % tiles_here of head s / tiles_here.
+  auto load_step = [&](int s) {
+    const int h = FORM == kWideAlone ? s / tiles_here : 0, tile = tile0 + s - h * tiles_here;
+    const T* kbase = static_cast<const T*>(a.k) + doc.k0 * a.k_tok + (kvh0 + h) * a.k_head;
+    const T* vbase = static_cast<const T*>(a.v) + doc.k0 * a.v_tok + (kvh0 + h) * a.v_head;
+    uint8_t* st = sStage + s % kStages * L::kStage;
+    const uint32_t sk = static_cast<uint32_t>(__cvta_generic_to_shared(st));
+    constexpr int kC = DP / 8;
+    if constexpr (kThreads % kC == 0) {  // a thread's pieces are a column: one pointer each to step on
+      constexpr int kStep = kThreads / kC;
+      const int r = threadIdx.x / kC, c = threadIdx.x % kC;
+      const int left = c < chunks ? klen - tile * kMmaKeys - r : 0;
+      const T* kp = kbase + (static_cast<long long>(tile) * kMmaKeys + r) * a.k_tok + c * 8;
+      const T* vp = vbase + (static_cast<long long>(tile) * kMmaKeys + r) * a.v_tok + c * 8;
+      const long long k_step = kStep * a.k_tok, v_step = kStep * a.v_tok;
+      const uint32_t to = sk + r * L::kRow + c * 16;
+#pragma unroll
+      for (int j = 0; j < kMmaKeys / kStep; ++j) {
+        const bool take = j * kStep < left;
+        cp_async16(to + j * kStep * L::kRow, take ? kp : kbase, take);
+        cp_async16(to + j * kStep * L::kRow + L::kTile, take ? vp : vbase, take);
+        kp += k_step, vp += v_step;
+      }
+    } else {
+      for (int i = threadIdx.x; i < kMmaKeys * kC; i += kThreads) {
+        const int r = i / kC, c = i % kC;
+        const int key = tile * kMmaKeys + r;
+        const bool take = key < klen && c < chunks;
+        const long long kk = take ? key : 0;
+        const int cc = take ? c * 8 : 0;
+        cp_async16(sk + r * L::kRow + c * 16, kbase + kk * a.k_tok + cc, take);
+        cp_async16(sk + L::kTile + r * L::kRow + c * 16, vbase + kk * a.v_tok + cc, take);
+      }
+    }
+    if (FORM == kWideAlone && tile == tile0) load_queries(st + L::kStageQ, kvh0 + h);
+    if (a.axes) {
+      float* sp = reinterpret_cast<float*>(st + L::kPos);
+      for (int i = threadIdx.x; i < a.axes * kMmaKeys; i += kThreads) {
+        const int ax = i / kMmaKeys, key = tile * kMmaKeys + i % kMmaKeys;
+        sp[i] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
+      }
+    }
+  };
+
+  if constexpr (FORM != kWideAlone) load_queries(sQ, kvh0);
 #pragma unroll
   for (int p = 0; p < kStages - 1; ++p) {
-    if (tile0 + p < tile1) load_tile(tile0 + p);
+    if (p < steps) load_step(p);
     cp_async_commit();
   }
 
@@ -191,36 +226,64 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
   for (int e = 0; e < 2; ++e) {
     const int r = min(wrow + g + 8 * e, rows - 1);
     hi[e] = hi_of(r);
-    const int row = item.row0 + r;
-    const int h = kvh * a.group + row % a.group;
 #pragma unroll
-    for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
-      slope[e][ax] = ax < a.axes ? a.slopes[h * a.axes + ax] : 0.f;
-      qpos[e][ax] = ax < a.axes ? a.q_pos[ax * a.q_total + doc.q0 + row / a.group] : 0.f;
+    for (int ax = 0; ax < kAttnMaxAxes; ++ax)
+      qpos[e][ax] = ax < a.axes ? a.q_pos[ax * a.q_total + doc.q0 + (item.row0 + r) / a.group] : 0.f;
+  }
+  auto load_slopes = [&](int kvh) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int h = kvh * a.group + (item.row0 + min(wrow + g + 8 * e, rows - 1)) % a.group;
+#pragma unroll
+      for (int ax = 0; ax < kAttnMaxAxes; ++ax) slope[e][ax] = ax < a.axes ? a.slopes[h * a.axes + ax] : 0.f;
     }
+  };
+  load_slopes(kvh0);
+
+  float o[DP / 8][4], m[2], l[2];
+  auto reset = [&] {
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
+  };
+  reset();
+  auto place = [&](int kvh, int r, int c) {  // of 8 elements of the output
+    const int row = item.row0 + r;
+    return reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
+                                    (static_cast<long long>(doc.q0) + row / a.group) * a.o_tok +
+                                    (kvh * a.group + row % a.group) * a.o_head + c * 8);
+  };
+  auto join_lanes = [&] {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+  };
+  if (FORM == kWideAlone && steps == 0) {  // no row sees a key: zeros
+    for (int i = threadIdx.x; i < heads * rows * chunks; i += kThreads)
+      *place(kvh0 + i / (rows * chunks), i / chunks % rows, i % chunks) = make_uint4(0, 0, 0, 0);
+    return;
   }
 
-  float o[DP / 8][4];
-#pragma unroll
-  for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
   uint32_t qf[kKD][4];
-  for (int tile = tile0; tile < tile1; ++tile) {
+  int tile = tile0;
+  for (int step = 0; step < steps; ++step) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    if (tile + kStages - 1 < tile1) load_tile(tile + kStages - 1);
+    if (step + kStages - 1 < steps) load_step(step + kStages - 1);
     cp_async_commit();
+    uint8_t* st = sStage + step % kStages * L::kStage;
     if (tile == tile0) {
-      const uint32_t sq = static_cast<uint32_t>(__cvta_generic_to_shared(sQ));
+      const uint32_t sq =
+          static_cast<uint32_t>(__cvta_generic_to_shared(FORM == kWideAlone ? st + L::kStageQ : sQ));
 #pragma unroll
       for (int kd = 0; kd < kKD; ++kd)
         ldmatrix4(qf[kd], sq + (wrow + (lane & 15)) * L::kRow + kd * 32 + (lane >> 4) * 16);
     }
-    const uint8_t* st = sStage + (tile - tile0) % kStages * L::kStage;
     const uint32_t sk = static_cast<uint32_t>(__cvta_generic_to_shared(st));
     const uint32_t sv = sk + L::kTile;
-    const float* sp = reinterpret_cast<const float*>(st + 2 * L::kTile);
+    const float* sp = reinterpret_cast<const float*>(st + L::kPos);
     const int wk0 = FEW ? warp * kWarpKeys : 0;  // this warp's first key within the tile
     const int key0 = tile * kMmaKeys + wk0;
 
@@ -237,11 +300,16 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
         mma<T>(s[n], qf[kd], b[0], b[1]);
         mma<T>(s[n + 1], qf[kd], b[2], b[3]);
       }
-    if (a.cap_log2 > 0.f) {
+    if (a.cap_log2 > kSeriesCap * 1.44269504f) {
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped(s[n][e], a);
+        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped<kCapSeries>(s[n][e], a);
+    } else if (a.cap_log2 > 0.f) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped<kCapExp>(s[n][e], a);
     } else {
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
@@ -278,12 +346,12 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float base = top == -INFINITY ? 0.f : top;  // a row that has seen nothing yet
-      const float shrink = exp2_fast(m[e] - base);
+      const float shrink = exp2_fast(m[e] - base), lift = base - kWeightShift;
       m[e] = top;
       float sum = 0.f;
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
-        const float p0 = exp2_fast(s[n][2 * e] - base), p1 = exp2_fast(s[n][2 * e + 1] - base);
+        const float p0 = exp2_fast(s[n][2 * e] - lift), p1 = exp2_fast(s[n][2 * e + 1] - lift);
         sum += p0 + p1;
         pf[n][e] = pack2<T>(p0, p1);
       }
@@ -306,24 +374,45 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
         mma<T>(o[i + 1], pa, b[2], b[3]);
       }
     }
+    ++tile;
+    if (FORM == kWideAlone && tile == tile1) {
+      // A head's last tile. A warp's rows go out through the places of its own queries, which
+      // it has in registers (those of the first tile's stage, or the unused ones of this).
+      const int h = kvh0 + step / tiles_here;
+      join_lanes();
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];  // a row that sees nothing is zeros
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+          *reinterpret_cast<uint32_t*>(st + L::kStageQ + (wrow + g + 8 * e) * L::kRow + i * 16 + t4 * 4) =
+              pack2<T>(o[i][2 * e] * inv, o[i][2 * e + 1] * inv);
+      }
+      __syncwarp();
+      for (int i = lane; i < 16 * chunks; i += 32) {
+        const int r = wrow + i / chunks, c = i % chunks;
+        if (r < rows) *place(h, r, c) = *reinterpret_cast<const uint4*>(st + L::kStageQ + r * L::kRow + c * 16);
+      }
+      tile = tile0;
+      if (step + 1 < steps) {
+        load_slopes(h + 1);
+        reset();
+      }
+    }
   }
   cp_async_wait<0>();
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-  }
+  if constexpr (FORM == kWideAlone) return;
+  const int kvh = kvh0;
+  join_lanes();
 
   auto store8 = [&](int r, int c, const float (&f)[8]) {
-    const int row = item.row0 + r;
-    T* dst = static_cast<T*>(a.out) + (static_cast<long long>(doc.q0) + row / a.group) * a.o_tok +
-             (kvh * a.group + row % a.group) * a.o_head + c * 8;
     uint4 u;
     u.x = pack2<T>(f[0], f[1]);
     u.y = pack2<T>(f[2], f[3]);
     u.z = pack2<T>(f[4], f[5]);
     u.w = pack2<T>(f[6], f[7]);
-    *reinterpret_cast<uint4*>(dst) = u;
+    *place(kvh, r, c) = u;
   };
 
   // Partial results of the warps, 16 rows each, in the place of the stages.
@@ -403,16 +492,28 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const __grid_constan
   if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <typename T, int DP, bool FEW>
-cudaError_t launch(const AttnArgs& a, int cluster, cudaStream_t s) {
-  auto fn = attn_mma_kernel<T, DP, FEW>;
+template <typename T, int DP, int FORM>
+cudaError_t launch(const AttnArgs& a, int cluster, int tiles, cudaStream_t s) {
+  auto fn = attn_mma_kernel<T, DP, FORM>;
   static AttrOnce once;
-  const cudaError_t e = once.set(reinterpret_cast<const void*>(fn), Layout<DP, FEW>::kBytes, true);
+  cudaError_t e = once.set(reinterpret_cast<const void*>(fn), Layout<DP, FORM>::bytes(kStages), true);
   if (e != cudaSuccess) return e;
+  if constexpr (FORM == kWideAlone) {
+    // Several heads to a CTA, so that one's loads run under another's work, while that leaves
+    // some CTAs for every place; and no more stages than it has steps.
+    AttnArgs b = a;
+    b.heads_per_block = static_cast<int>(
+        std::clamp<long long>(static_cast<long long>(a.num_items) * a.kv_heads / (12LL * a.num_sms), 1, a.kv_heads));
+    const long long steps = static_cast<long long>(tiles) * b.heads_per_block;
+    const int smem = Layout<DP, FORM>::bytes(static_cast<int>(std::clamp<long long>(steps, 1, kStages)));
+    const dim3 grid(a.num_items, (a.kv_heads + b.heads_per_block - 1) / b.heads_per_block);
+    fn<<<grid, kThreads, smem, s>>>(b);
+    return cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.num_items) * cluster, a.kv_heads);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Layout<DP, FEW>::kBytes;
+  cfg.dynamicSmemBytes = Layout<DP, FORM>::bytes(kStages);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -423,20 +524,25 @@ cudaError_t launch(const AttnArgs& a, int cluster, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
-template <typename T, bool FEW>
-cudaError_t by_dim(const AttnArgs& a, int cluster, cudaStream_t s) {
-  if (a.head_dim <= 32) return launch<T, 32, FEW>(a, cluster, s);
-  if (a.head_dim <= 64) return launch<T, 64, FEW>(a, cluster, s);
-  if (a.head_dim <= 96) return launch<T, 96, FEW>(a, cluster, s);
-  return launch<T, 128, FEW>(a, cluster, s);
+template <typename T, int FORM>
+cudaError_t by_dim(const AttnArgs& a, int cluster, int tiles, cudaStream_t s) {
+  if (a.head_dim <= 32) return launch<T, 32, FORM>(a, cluster, tiles, s);
+  if (a.head_dim <= 64) return launch<T, 64, FORM>(a, cluster, tiles, s);
+  if (a.head_dim <= 96) return launch<T, 96, FORM>(a, cluster, tiles, s);
+  return launch<T, 128, FORM>(a, cluster, tiles, s);
+}
+
+template <typename T>
+cudaError_t by_form(const AttnArgs& a, bool few_rows, int cluster, int tiles, cudaStream_t s) {
+  if (few_rows) return by_dim<T, kFew>(a, cluster, tiles, s);
+  return cluster > 1 ? by_dim<T, kWideShared>(a, cluster, tiles, s) : by_dim<T, kWideAlone>(a, cluster, tiles, s);
 }
 
 }  // namespace
 
-cudaError_t attn_mma_launch(const AttnArgs& a, int dtype, bool few_rows, int cluster, cudaStream_t s) {
-  if (dtype == kTokenBf16)
-    return few_rows ? by_dim<__nv_bfloat16, true>(a, cluster, s) : by_dim<__nv_bfloat16, false>(a, cluster, s);
-  return few_rows ? by_dim<__half, true>(a, cluster, s) : by_dim<__half, false>(a, cluster, s);
+cudaError_t attn_mma_launch(const AttnArgs& a, int dtype, bool few_rows, int cluster, int tiles, cudaStream_t s) {
+  return dtype == kTokenBf16 ? by_form<__nv_bfloat16>(a, few_rows, cluster, tiles, s)
+                             : by_form<__half>(a, few_rows, cluster, tiles, s);
 }
 
 }  // namespace ah

@@ -109,7 +109,7 @@ __device__ __forceinline__ void weights32(const uint32_t (&u)[32], uint64_t mul,
   }
 }
 
-template <typename T, int NCH, bool CAP, bool BIAS>
+template <typename T, int NCH, int CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ AttnTcArgs args) {
   using L = Smem<NCH>;
   const AttnArgs& a = args.a;
@@ -345,13 +345,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     };
     auto meet = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + g) : "memory"); };  // the tile's eight warps
     float* poss = reinterpret_cast<float*>(smem + L::kPos) + g * 2 * kAttnMaxAxes * kTcKeys;
-    // The positions of the keys of tile j, into the buffer of j: written before the meeting of
-    // tile j, read after it.
+    // The negated positions of the keys of tile j, into the buffer of j: written before the
+    // meeting of tile j, read after it.
     auto stage_positions = [&](int j) {
       const int t = threadIdx.x & 255, key = j * kTcKeys + (t & 127);
       float* put = poss + (j & 1) * kAttnMaxAxes * kTcKeys;
       for (int ax = t >> 7; ax < a.axes; ax += 2)
-        put[ax * kTcKeys + (t & 127)] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
+        put[ax * kTcKeys + (t & 127)] = key < klen ? -a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
     };
     const float mul = CAP || BIAS ? 1.f : a.score_mul;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2];
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           float v = __uint_as_float(x[e]);
-          if constexpr (CAP)
-            v = attn_capped(v, a);
+          if constexpr (CAP != kCapNone)
+            v = attn_capped<CAP>(v, a);
           else
             v *= a.score_mul;
           x[e] = __float_as_uint(v);
@@ -372,14 +372,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
           for (int ax = 0; ax < kAttnMaxAxes; ++ax) {
             if (ax >= a.axes) break;
+            const uint64_t fall = ptx::pack_f2(-slope[ax], -slope[ax]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float2 kp = *reinterpret_cast<const float2*>(pos + ax * kTcKeys + k * 8);
+              const uint64_t away = *reinterpret_cast<const uint64_t*>(pos + ax * kTcKeys + k * 8);  // negated
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t* y = x + 4 * k + 2 * e;
-                y[0] = __float_as_uint(__uint_as_float(y[0]) - slope[ax] * fabsf(qpos[e][ax] - kp.x));
-                y[1] = __float_as_uint(__uint_as_float(y[1]) - slope[ax] * fabsf(qpos[e][ax] - kp.y));
+                const float2 far = ptx::unpack_f2(ptx::add_f2(ptx::pack_f2(qpos[e][ax], qpos[e][ax]), away));
+                const float2 z = ptx::unpack_f2(
+                    ptx::fma_f2(ptx::pack_f2(fabsf(far.x), fabsf(far.y)), fall,
+                                ptx::pack_f2(__uint_as_float(y[0]), __uint_as_float(y[1]))));
+                y[0] = __float_as_uint(z.x), y[1] = __float_as_uint(z.y);
               }
             }
           }
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   if (threadIdx.x == 0 && *abort_flag) atomicOr(a.status, 1u);
 }
 
-template <typename T, int NCH, bool CAP, bool BIAS>
+template <typename T, int NCH, int CAP, bool BIAS>
 cudaError_t launch(const AttnTcArgs& args, cudaStream_t s) {
   auto fn = attn_tc_kernel<T, NCH, CAP, BIAS>;
   static AttrOnce once;
@@ -535,11 +539,18 @@ cudaError_t launch(const AttnTcArgs& args, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+template <typename T, int NCH, int CAP>
+cudaError_t launch_biased(const AttnTcArgs& args, cudaStream_t s) {
+  return args.a.axes > 0 ? launch<T, NCH, CAP, true>(args, s) : launch<T, NCH, CAP, false>(args, s);
+}
+
 template <typename T, int NCH>
 cudaError_t launch_variant(const AttnTcArgs& args, cudaStream_t s) {
-  const bool cap = args.a.cap_log2 > 0.f, bias = args.a.axes > 0;
-  if (cap) return bias ? launch<T, NCH, true, true>(args, s) : launch<T, NCH, true, false>(args, s);
-  return bias ? launch<T, NCH, false, true>(args, s) : launch<T, NCH, false, false>(args, s);
+  switch (cap_form(args.a)) {
+    case kCapExp: return launch_biased<T, NCH, kCapExp>(args, s);
+    case kCapSeries: return launch_biased<T, NCH, kCapSeries>(args, s);
+    default: return launch_biased<T, NCH, kCapNone>(args, s);
+  }
 }
 
 // One translation unit each (attn_tc_*.cu).

@@ -9,21 +9,36 @@
 
 namespace ah {
 
+// How scores are capped, cap * tanh(s / cap), in powers of two:
+//   kCapExp     cap (1 - 2 / (1 + exp(2 s / cap))), good to a few units of 2^-24 cap
+//   kCapSeries  for a cap beyond 256, where that is no longer small beside the score: small
+//               arguments take the odd series of tanh instead
+enum CapForm : int { kCapNone = 0, kCapExp = 1, kCapSeries = 2 };
 constexpr float kSeriesCap = 256.f;
 
-// cap * tanh(s / cap) in powers of two: cap (1 - 2 / (1 + exp(2 s / cap))), good to a few units
-// of 2^-24 cap. Beyond a cap of 256, where that is no longer small beside the score, small
-// arguments take the odd series of tanh instead.
+inline CapForm cap_form(const AttnArgs& a) {
+  return a.cap_log2 > kSeriesCap * 1.44269504f ? kCapSeries : (a.cap_log2 > 0.f ? kCapExp : kCapNone);
+}
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int FORM>
 __device__ __forceinline__ float attn_capped(float s, const AttnArgs& a) {
-  const float u = s * a.cap_arg;
-  if (a.cap_log2 > kSeriesCap * 1.44269504f && fabsf(u) < 0.3f) {
-    // tanh u = u - u^3/3 + 2u^5/15 - 17u^7/315 + 62u^9/2835; the next term is below 2^-24 u
-    const float z = u * u;
-    return a.cap_log2 * u * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835)))));
-  }
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * 2.88539008f));
-  return a.cap_log2 - __fdividef(2.f * a.cap_log2, 1.f + e);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(s * a.cap_exp));
+  const float x = a.cap_log2 - 2.f * a.cap_log2 * rcp_fast(1.f + e);
+  if constexpr (FORM == kCapSeries) {
+    // tanh u = u - u^3/3 + 2u^5/15 - 17u^7/315 + 62u^9/2835; the next term is below 2^-24 u
+    const float u = s * a.cap_arg, z = u * u;
+    const float t =
+        a.cap_log2 * u * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835)))));
+    return fabsf(u) < 0.3f ? t : x;
+  }
+  return x;
 }
 
 // A kernel's function attributes, set once per device.

@@ -103,18 +103,20 @@ struct AttnArgs {
   const AttnItem* items = nullptr;
   const float* slopes = nullptr;  // [q heads][axes], times log2(e)
   uint32_t* status = nullptr;
-  int num_items = 0;
+  int num_items = 0, num_sms = 148;
+  int heads_per_block = 1;  // set by the launch that uses it
   int q_heads = 0, kv_heads = 0, group = 1, head_dim = 0, axes = 0, causal = 0;
   // Scores in powers of two: x = score_mul * (q.k), or with a cap
-  // x = cap_log2 * tanh(cap_arg * (q.k)).
-  float score_mul = 0.f, cap_log2 = 0.f, cap_arg = 0.f;
+  // x = cap_log2 * tanh(cap_arg * (q.k)), with cap_exp = 2 log2(e) cap_arg.
+  float score_mul = 0.f, cap_log2 = 0.f, cap_arg = 0.f, cap_exp = 0.f;
 };
 
 // Rows per block of the two forms of the mma.sync kernel.
 constexpr int kMmaRowsWide = 64;  // four warps of 16 rows
 constexpr int kMmaRowsFew = 16;   // 16 rows, the keys shared out over the warps
 constexpr int kMmaKeys = 64;      // keys per tile
-cudaError_t attn_mma_launch(const AttnArgs& a, int dtype, bool few_rows, int cluster, cudaStream_t s);
+// `tiles`: the most key tiles of any block.
+cudaError_t attn_mma_launch(const AttnArgs& a, int dtype, bool few_rows, int cluster, int tiles, cudaStream_t s);
 
 // attn_tc.cu: tcgen05 form. Its items are not rows but query tokens: two tiles of 128, one
 // after the other of one query head, or, for an even group, of the same tokens for two heads.

@@ -63,7 +63,7 @@ namespace ah {
 cudaError_t norm_launch(const NormArgs&, int, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
 cudaError_t rope_launch(const RopeTable&, const RopeArgs&, int, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
 cudaError_t attn_tc_launch(const AttnArgs&, int, cudaStream_t, std::string*) { ++g_launches; return cudaSuccess; }
-cudaError_t attn_mma_launch(const AttnArgs&, int, bool, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
+cudaError_t attn_mma_launch(const AttnArgs&, int, bool, int, int, cudaStream_t) { ++g_launches; return cudaSuccess; }
 }
 """
 
