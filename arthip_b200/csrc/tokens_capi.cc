@@ -149,10 +149,55 @@ bool Overlap(const View& a, const View& b) {
 
 bool Aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// Which documents the tcgen05 kernel takes: those that fill more than half of its tiles of 128
-// queries and one tile of keys. At 64 queries and keys (2040 windows, 6 heads of 32) it takes
-// the mma.sync kernel 125 us; at 32400 of both (8 heads of 64) 8.2 ms against 4.4 ms here.
-bool UseTensorMemory(const ah::AttnDoc& doc) { return doc.nq > ah::kTcRows / 2 && doc.nk >= ah::kTcKeys; }
+int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Which documents the tcgen05 kernel takes and which the mma.sync kernel: the one that is
+// expected to be done sooner. A CTA's time on an SM, in us, is about
+//   tcgen05   start + tile * (tiles of 128 keys), for 256 rows
+//   mma.sync  start + tile * (tiles of 64 keys), for 64 rows, with the SM full of CTAs
+// with the constants below, by width of the head, from equal documents of 65 to 512 tokens
+// (131072 in all, 4 heads). They meet at about 400 tokens of 32 elements (384: 236 us here, 220
+// us there; 512: 253 and 284), 150 of 64 (128: 160 and 135; 160: 199 and 211) and 70 of 128
+// (65: 610 and 588; 96: 269 and 439). Where the tcgen05 kernel's few large CTAs leave SMs empty,
+// its time does not fall, while the mma.sync kernel cuts its keys up further, at about 1.7 times
+// the work and 8 us for the joining: 1024 queries on 8192 keys, 4 heads of 64, 111 us and 59;
+// 1024 on 1024, 12 heads of 64, 23 and 33.
+class KernelChoice {
+ public:
+  KernelChoice(const std::vector<ah::AttnDoc>& docs, int q_heads, int kv_heads, int head_dim, int num_sms)
+      : group_(q_heads / kv_heads), q_heads_(q_heads), kv_heads_(kv_heads), num_sms_(num_sms) {
+    static constexpr Cost kCosts[3] = {{4.7, 3.0, 0.65, 0.56}, {3.4, 2.3, 1.2, 0.62}, {4.1, 3.4, 3.1, 1.41}};
+    cost_ = kCosts[head_dim <= 32 ? 0 : (head_dim <= 64 ? 1 : 2)];
+    for (const ah::AttnDoc& d : docs) {
+      if (!Candidate(d)) continue;
+      tc_ctas_ += TcCtas(d);
+      mma_blocks_ += MmaBlocks(d);
+      ++candidates_;
+    }
+  }
+  bool TensorMemory(const ah::AttnDoc& d) const {
+    if (!Candidate(d)) return false;
+    const double tc = TcCtas(d) * (cost_.tc_start + cost_.tc_tile * CeilDiv(d.nk, ah::kTcKeys));
+    double mma = MmaBlocks(d) * (cost_.mma_start + cost_.mma_tile * CeilDiv(d.nk, ah::kMmaKeys)) / num_sms_;
+    if (mma_blocks_ < 8 * num_sms_) mma = 1.7 * mma + 8.0 / candidates_;
+    return tc / std::min<int64_t>(num_sms_, tc_ctas_) < mma;
+  }
+
+ private:
+  struct Cost {
+    double tc_start, tc_tile, mma_start, mma_tile;
+  };
+  bool Candidate(const ah::AttnDoc& d) const { return d.nk > 0 && int64_t{d.nq} * group_ > ah::kMmaRowsFew; }
+  int64_t TcCtas(const ah::AttnDoc& d) const {
+    return CeilDiv(d.nq, ah::attn_tc_item_tokens(group_)) * (ah::attn_tc_head_pairs(group_) ? q_heads_ / 2 : q_heads_);
+  }
+  int64_t MmaBlocks(const ah::AttnDoc& d) const {
+    return CeilDiv(int64_t{d.nq} * group_, ah::kMmaRowsWide) * kv_heads_;
+  }
+  int group_, q_heads_, kv_heads_, num_sms_;
+  Cost cost_;
+  int64_t tc_ctas_ = 0, mma_blocks_ = 0, candidates_ = 0;
+};
 
 View Floats(const float* p, int64_t n) { return View{p, 1, 0, 1, 0, 2 * n}; }
 
@@ -456,6 +501,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
     a.score_mul = static_cast<float>(d->scale * kLog2e);
   }
   // Blocks of rows, those with the most keys first, so that the last ones to start are short.
+  const KernelChoice choice(table, d->q_heads, d->kv_heads, d->head_dim, h->num_sms);
   std::vector<ah::AttnItem> few, wide, tc;
   int few_tiles = 0, wide_tiles = 0;
   std::vector<int> order(docs);
@@ -463,7 +509,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return table[i].nk > table[j].nk; });
   for (int i : order) {
     const ah::AttnDoc& doc = table[i];
-    if (UseTensorMemory(doc)) {
+    if (choice.TensorMemory(doc)) {
       const int step = ah::attn_tc_item_tokens(group);
       for (int r = (doc.nq - 1) / step * step; r >= 0; r -= step) tc.push_back({i, r});  // causal: longest first
       continue;
