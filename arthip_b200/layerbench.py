@@ -1,8 +1,15 @@
 """Single conv layer benchmark (the 64->64 + bias + ReLU microbench on a 1080x1920 NHWC frame
-by default), through the ``ah_conv3x3_*`` C ABI.
+by default), through the ``ah_conv3x3_*`` C ABI, or single token operator over the same frame
+(``--op norm | rope | attention``, ``ah_norm_*`` / ``ah_rope_*`` / ``ah_attn_*``).
 
     python -m arthip_b200.layerbench [--C 64 --M 64 --H 1080 --W 1920 --act 1 --adds 0]
                                      [--warmup 3 --iters 20] [--algo direct|winograd]
+    python -m arthip_b200.layerbench --op attention [--C 64 --H 1080 --W 1920 --head-dim 32 --window 8]
+
+Of the token operators, ``norm`` is the RMS norms before and after a block with its layer scale
+over H x W pixels of C channels; ``rope`` turns q and k of C / head-dim heads by row and column;
+``attention`` is that many heads over windows of window x window pixels with a distance bias by
+row and column (``--window 0``: the whole frame as one document).
 
 Prints one JSON line: mean launch time from CUDA events around `iters` back-to-back
 launches on the current stream, the algorithmic direct-conv FLOPs (2*9*C*M*H*W) and bytes
@@ -54,9 +61,15 @@ def main(argv=None) -> int:
     ap.add_argument("--model", choices=["C4F32", "R8F64", "R16F96"],
                     help="time whole frames of this BASELINE chain (luma, 2x) at --H x --W through the "
                          "engine's CUDA graph instead of one layer (a small-frame case for profilers)")
+    ap.add_argument("--op", choices=["conv", "norm", "rope", "attention"], default="conv",
+                    help="the conv layer, or a token operator over the frame")
+    ap.add_argument("--head-dim", type=int, default=32, help="elements per attention head (--op rope, attention)")
+    ap.add_argument("--window", type=int, default=8, help="side of the attention windows; 0: the whole frame")
     args = ap.parse_args(argv)
     if args.model:
         return _model_frames(args)
+    if args.op != "conv":
+        return _token_operator(args, ap)
 
     import torch
 
@@ -106,6 +119,86 @@ def main(argv=None) -> int:
         "tflops_frac": tflops / peaks["bf16_tflops"], "peaks": src, "iters": args.iters, "status": status,
     }))
     conv.close()
+    return 0 if status == 0 else 1
+
+
+def _token_operator(args, ap) -> int:
+    import torch
+
+    from arthip_b200.token_ops import AxisRotary, TokenAttention, TokenNorm
+
+    C, H, W, d = args.C, args.H, args.W, args.head_dim
+    n = H * W
+    g = torch.Generator(device="cuda").manual_seed(args.seed)
+
+    def tensor(channels):
+        return torch.randn(n, channels, generator=g, device="cuda", dtype=torch.float16)
+
+    s = torch.cuda.current_stream().cuda_stream
+    status = 0
+    if args.op == "norm":
+        x, y, out, norm = tensor(C), tensor(C), tensor(C), tensor(C)
+        w = np.ones(C, dtype=np.float32)
+        op = TokenNorm(C, post_norm="rms", pre_norm="rms", post_weight=w, pre_weight=w, layer_scale=0.5 * w)
+        label, flops, nbytes = f"norm {C} {H}x{W}", 12.0 * n * C, 8.0 * n * C + 12.0 * C
+
+        def launch():
+            op.run(n, x.data_ptr(), out.data_ptr(), norm.data_ptr(), y.data_ptr(), stream=s)
+    else:
+        if C % d or d % 16:
+            ap.error("--C must be a multiple of --head-dim, and that of 16")
+        heads = C // d
+        yy, xx = torch.meshgrid(torch.arange(H, device="cuda"), torch.arange(W, device="cuda"), indexing="ij")
+        if args.op == "rope":
+            q, k, q_out, k_out = tensor(C), tensor(C), tensor(C), tensor(C)
+            pos = torch.stack([yy.flatten(), xx.flatten()]).float().contiguous()
+            op = AxisRotary(d, [d // 2, d // 2])
+            label, flops, nbytes = f"rope {heads}x{d} {H}x{W}", 6.0 * n * C, 8.0 * n * C + 8.0 * n
+
+            def launch():
+                op.run(n, pos.data_ptr(), q.data_ptr(), heads, q_out.data_ptr(), k.data_ptr(), heads,
+                       k_out.data_ptr(), stream=s)
+        else:
+            b = args.window
+            if b < 0 or (b and (H % b or W % b)):
+                ap.error("--window must divide --H and --W")
+
+            def windows(t):  # tokens of one window after those of another
+                return t.flatten() if b == 0 else t.view(H // b, b, W // b, b).permute(0, 2, 1, 3).reshape(-1)
+
+            pos = torch.stack([windows(yy), windows(xx)]).float().contiguous()
+            q, k, v, out = tensor(C), tensor(C), tensor(C), tensor(C)
+            each = b * b if b else n
+            off = np.arange(0, n + 1, each)
+            op = TokenAttention(off, off, heads, heads, d, slopes=np.full((heads, 2), 0.05, dtype=np.float32))
+            label = f"attention {heads}x{d} {'whole' if b == 0 else f'{b}x{b} windows'} {H}x{W}"
+            flops, nbytes = 4.0 * n * each * C, 8.0 * n * C + 16.0 * n
+
+            def launch():
+                op.run(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pos.data_ptr(), pos.data_ptr(),
+                       stream=s)
+
+    for _ in range(max(1, args.warmup)):
+        launch()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    for _ in range(args.iters):
+        launch()
+    e1.record()
+    torch.cuda.synchronize()
+    if args.op == "attention":
+        status = op.status()
+    ms = e0.elapsed_time(e1) / args.iters
+    peaks, src = _peaks()
+    roof_ms = max(flops / (peaks["bf16_tflops"] * 1e12), nbytes / (peaks["hbm_gbs"] * 1e9)) * 1e3
+    print(json.dumps({
+        "layer": label, "us_per_launch": ms * 1e3, "tflops": flops / (ms * 1e-3) / 1e12,
+        "gbs": nbytes / (ms * 1e-3) / 1e9, "algorithmic_flops": flops, "algorithmic_bytes": nbytes,
+        "roofline_us": roof_ms * 1e3, "roofline_frac": roof_ms / ms, "peaks": src, "iters": args.iters,
+        "status": status,
+    }))
+    op.close()
     return 0 if status == 0 else 1
 
 

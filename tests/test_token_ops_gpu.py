@@ -482,6 +482,16 @@ def test_run_refusals_launch_nothing():
     assert (out == 7).all() and (q == 0).all()
 
 
+@pytest.mark.parametrize("args", [["--op", "norm"], ["--op", "rope"], ["--op", "attention"],
+                                  ["--op", "attention", "--window", "0"]])
+def test_layerbench_times_the_operators(args, capsys):
+    import json
+    from arthip_b200 import layerbench
+    assert layerbench.main(args + ["--C", "96", "--H", "40", "--W", "64", "--iters", "2"]) == 0
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert line["us_per_launch"] > 0 and line["algorithmic_bytes"] > 0 and line["status"] == 0
+
+
 # ---------------------------------------------------------------------------
 # A token block between conv layers
 # ---------------------------------------------------------------------------
