@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
   auto hi_of = [&](int r) {
     if (!a.causal) return klen;
     const int tok = (item.row0 + r) / a.group;
-    return min(klen, max(prefix, tok + klen - doc.nq + 1));
+    return min(klen, max(prefix, klen - (doc.nq - tok) + 1));
   };
   const int hi_last = max(hi_of(rows - 1), 0);   // the largest
   const int hi_first = hi_of(0);                 // the smallest

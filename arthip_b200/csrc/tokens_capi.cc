@@ -164,8 +164,8 @@ int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // 1024 on 1024, 12 heads of 64, 23 and 33.
 class KernelChoice {
  public:
-  KernelChoice(const std::vector<ah::AttnDoc>& docs, int q_heads, int kv_heads, int head_dim, int num_sms)
-      : group_(q_heads / kv_heads), q_heads_(q_heads), kv_heads_(kv_heads), num_sms_(num_sms) {
+  KernelChoice(const std::vector<ah::AttnDoc>& docs, int algo, int q_heads, int kv_heads, int head_dim, int num_sms)
+      : algo_(algo), group_(q_heads / kv_heads), q_heads_(q_heads), kv_heads_(kv_heads), num_sms_(num_sms) {
     static constexpr Cost kCosts[3] = {{4.7, 3.0, 0.65, 0.56}, {3.4, 2.3, 1.2, 0.62}, {4.1, 3.4, 3.1, 1.41}};
     cost_ = kCosts[head_dim <= 32 ? 0 : (head_dim <= 64 ? 1 : 2)];
     for (const ah::AttnDoc& d : docs) {
@@ -176,6 +176,7 @@ class KernelChoice {
     }
   }
   bool TensorMemory(const ah::AttnDoc& d) const {
+    if (algo_ != 0) return algo_ == 2 && d.nq > 0 && d.nk > 0;
     if (!Candidate(d)) return false;
     const double tc = TcCtas(d) * (cost_.tc_start + cost_.tc_tile * CeilDiv(d.nk, ah::kTcKeys));
     double mma = MmaBlocks(d) * (cost_.mma_start + cost_.mma_tile * CeilDiv(d.nk, ah::kMmaKeys)) / num_sms_;
@@ -194,7 +195,7 @@ class KernelChoice {
   int64_t MmaBlocks(const ah::AttnDoc& d) const {
     return CeilDiv(int64_t{d.nq} * group_, ah::kMmaRowsWide) * kv_heads_;
   }
-  int group_, q_heads_, kv_heads_, num_sms_;
+  int algo_, group_, q_heads_, kv_heads_, num_sms_;
   Cost cost_;
   int64_t tc_ctas_ = 0, mma_blocks_ = 0, candidates_ = 0;
 };
@@ -219,7 +220,7 @@ struct ah_rope {
 struct ah_attn {
   int device = 0, num_sms = 0, dtype = 0;
   ah::AttnArgs args;
-  int64_t q_total = 0, k_total = 0;
+  int64_t q_total = 0, k_total = 0, docs_n = 0;
   DeviceBuffer docs, few, wide, tc, slopes, status;
   int n_few = 0, n_wide = 0, n_tc = 0, few_cluster = 1, wide_cluster = 1, few_tiles = 0, wide_tiles = 0;
 };
@@ -458,6 +459,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
     return Fail("attention: scale / cap or cap is out of fp32 range", err, errlen);
   if (d->mask < 0 || d->mask > 1) return Fail("attention: unknown mask", err, errlen);
   if (prefix && d->mask != 1) return Fail("attention: a prefix needs the causal mask", err, errlen);
+  if (d->algo < 0 || d->algo > 2) return Fail("attention: unknown algo", err, errlen);
   if (d->axes < 0 || d->axes > ah::kAttnMaxAxes) return Fail("attention: 0 to 3 bias axes", err, errlen);
   if ((d->axes > 0) != (slopes != nullptr)) return Fail("attention: slopes go with bias axes", err, errlen);
   const int group = d->q_heads / d->kv_heads;
@@ -489,6 +491,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   h->dtype = d->dtype;
   h->q_total = q_offsets[docs];
   h->k_total = k_offsets[docs];
+  h->docs_n = docs;
   ah::AttnArgs& a = h->args;
   a.q_heads = d->q_heads, a.kv_heads = d->kv_heads, a.group = group, a.head_dim = d->head_dim;
   a.axes = d->axes, a.causal = d->mask;
@@ -501,7 +504,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
     a.score_mul = static_cast<float>(d->scale * kLog2e);
   }
   // Blocks of rows, those with the most keys first, so that the last ones to start are short.
-  const KernelChoice choice(table, d->q_heads, d->kv_heads, d->head_dim, h->num_sms);
+  const KernelChoice choice(table, d->algo, d->q_heads, d->kv_heads, d->head_dim, h->num_sms);
   std::vector<ah::AttnItem> few, wide, tc;
   int few_tiles = 0, wide_tiles = 0;
   std::vector<int> order(docs);
@@ -580,7 +583,8 @@ int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int e
   if (!o.distinct()) return Fail("attention: output heads or tokens overlap one another", err, errlen);
   const View qp = Floats(io->q_positions, h->q_total * h->args.axes);
   const View kp = Floats(io->k_positions, h->k_total * h->args.axes);
-  for (const View* t : {&q, &k, &v, &qp, &kp})
+  const View lens{io->k_lens, 1, 0, 1, 0, 2 * h->docs_n};
+  for (const View* t : {&q, &k, &v, &qp, &kp, &lens})
     if (Overlap(o, *t)) return Fail("attention: the output overlaps an input", err, errlen);
   DeviceScope scope(h->device);
   if (scope.error() != cudaSuccess) return CudaFail("attention: cudaSetDevice failed", scope.error(), err, errlen, 2);

@@ -27,6 +27,7 @@ _NORMS = {"none": 0, "rms": 1, "layer": 2}
 _GATES = {"none": 0, "sigmoid": 1, "tanh": 2, "silu": 3}
 _LAYOUTS = {"halves": 0, "pairs": 1, "shared": 2}
 _MASKS = {"full": 0, "causal": 1}
+_ALGOS = {"auto": 0, "mma": 1, "tc": 2}
 
 
 class _NormDesc(ctypes.Structure):
@@ -53,7 +54,7 @@ class _RopeIo(ctypes.Structure):
 
 class _AttnDesc(ctypes.Structure):
     _fields_ = [("dtype", _i32), ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("scale", _f32),
-                ("cap", _f32), ("mask", _i32), ("axes", _i32)]
+                ("cap", _f32), ("mask", _i32), ("axes", _i32), ("algo", _i32)]
 
 
 class _AttnIo(ctypes.Structure):
@@ -200,13 +201,15 @@ class TokenAttention(_Handle):
     ``mask``: "full", or "causal" (aligned to the last key), with ``prefix[i]`` first keys that
     every query of document i sees. ``cap``: scores become ``cap * tanh(score / cap)``.
     ``slopes`` [q_heads][axes]: ``slope * |q position - k position|`` is taken off the scores
-    for each axis. ``scale`` defaults to ``head_dim ** -0.5``."""
+    for each axis. ``scale`` defaults to ``head_dim ** -0.5``. ``algo``: "auto" takes for each
+    document the kernel that is expected to be done sooner; "mma" and "tc" the mma.sync and the
+    tcgen05 one for all."""
 
     _destroy = "ah_attn_destroy"
 
     def __init__(self, q_offsets, k_offsets, q_heads: int, kv_heads: int, head_dim: int, scale: float | None = None,
                  cap: float = 0.0, mask: str = "full", prefix=None, slopes=None, dtype: str = "fp16",
-                 device: int = 0):
+                 algo: str = "auto", device: int = 0):
         super().__init__()
         qo, ko = _whole(q_offsets, "q_offsets"), _whole(k_offsets, "k_offsets")
         if qo.size < 1 or qo.size != ko.size:
@@ -221,7 +224,8 @@ class TokenAttention(_Handle):
             axes = slopes.shape[1] if slopes.ndim == 2 else -1
             slopes = _floats(slopes, (q_heads, axes), "slopes")
         d = _AttnDesc(_code(_DTYPES, dtype, "dtype"), q_heads, kv_heads, head_dim,
-                      max(head_dim, 1) ** -0.5 if scale is None else scale, cap, _code(_MASKS, mask, "mask"), axes)
+                      max(head_dim, 1) ** -0.5 if scale is None else scale, cap, _code(_MASKS, mask, "mask"), axes,
+                      _code(_ALGOS, algo, "algo"))
         err = _err()
         self._check(self._lib.ah_attn_create(device, ctypes.byref(d), docs, qo.ctypes.data, ko.ctypes.data, _data(pre),
                                              _data(slopes), ctypes.byref(self._h), err, _ERR_LEN), err,

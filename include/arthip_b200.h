@@ -306,6 +306,8 @@ typedef struct {
   float cap;    /* 0 = none */
   int mask;
   int axes;     /* of the distance bias, 0..3 */
+  int algo;     /* 0: for each document the kernel that is expected to be done sooner;
+                 * 1: mma.sync for all; 2: tcgen05 for all that have queries and keys */
 } ah_attn_desc;
 /* q, out [q_offsets[docs]][q_heads][head_dim]; k, v [k_offsets[docs]][kv_heads][head_dim], by
  * strides that are multiples of 8 elements, from 16-byte aligned pointers; out overlaps no

@@ -202,7 +202,7 @@ def test_attention_create_refusals(fake):
                        ("offsets", dict(q_offsets=[], k_offsets=[])), ("whole", dict(q_offsets=[0.0, 4.0])),
                        ("slopes", dict(slopes=[1.0] * 4)), ("slopes", dict(slopes=[[1.0]] * 3)),
                        ("axes", dict(slopes=[[1.0] * 4] * 4)), ("finite", dict(slopes=[[math.inf]] * 4)),
-                       ("dtype", dict(dtype="fp8")), ("cudaSetDevice", dict(device=-1))]:
+                       ("dtype", dict(dtype="fp8")), ("algo", dict(algo="simt")), ("cudaSetDevice", dict(device=-1))]:
         refused(match, TokenAttention, **(good | bad))
     assert fake.fake_live() == 0
 
@@ -218,7 +218,8 @@ def test_attention_run_refusals(fake):
                        ("16-byte", dict(k_strides=(68, 64))), ("16-byte", dict(q_strides=(128, 60))),
                        ("stride", dict(v_strides=(-64, 64))), ("overlap one another", dict(out_strides=(64, 64))),
                        ("overlaps an input", dict(out_ptr=q)), ("overlaps an input", dict(out_ptr=k + 128)),
-                       ("overlaps an input", dict(out_ptr=p)), ("device 1", dict(stream=0x1000))]:
+                       ("overlaps an input", dict(out_ptr=p)),
+                       ("overlaps an input", dict(k_lens_ptr=o + 256)), ("device 1", dict(stream=0x1000))]:
         refused(match, op.run, **(ok | bad))
     assert fake.fake_launches() == before
     op.run(**ok)

@@ -245,17 +245,19 @@ def run_attn(qs, ks, hq=4, hk=2, d=64, dtype="fp16", causal=False, prefix=None, 
     if garbage:
         k[nk:], v[nk:] = math.nan, math.nan
     scale = d ** -0.5 if scale is None else scale
-    op = TokenAttention(qo, ko, hq, hk, d, scale=scale, cap=cap, mask="causal" if causal else "full", prefix=prefix,
-                        slopes=slopes, dtype=dtype)
-    op.run(ptr(q), ptr(k), ptr(v), ptr(out), ptr(q_pos), ptr(k_pos), ptr(dl), q.stride()[:2], k.stride()[:2],
-           v.stride()[:2], stream=stream())
-    torch.cuda.synchronize()
     ref, bound = attn_ref(q[:nq], k[:nk], v[:nk], qo, ko, scale, cap, causal, prefix, slopes, q_pos, k_pos, lens,
                           dtype)
-    check(out[:nq], ref, bound, dtype, "attention")
-    assert (out[nq:] == 7).all()
-    assert op.status() == 0
-    op.close()
+    for algo in ("auto", "mma", "tc"):  # the choice by expected time, and each kernel on everything
+        op = TokenAttention(qo, ko, hq, hk, d, scale=scale, cap=cap, mask="causal" if causal else "full",
+                            prefix=prefix, slopes=slopes, dtype=dtype, algo=algo)
+        out.fill_(7.0)
+        op.run(ptr(q), ptr(k), ptr(v), ptr(out), ptr(q_pos), ptr(k_pos), ptr(dl), q.stride()[:2], k.stride()[:2],
+               v.stride()[:2], stream=stream())
+        torch.cuda.synchronize()
+        check(out[:nq], ref, bound, dtype, f"attention ({algo})")
+        assert (out[nq:] == 7).all()
+        assert op.status() == 0
+        op.close()
 
 
 @pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 64, 72, 80, 96, 104, 128])
@@ -362,21 +364,22 @@ def test_attention_far_offsets():
     v = cache.as_strided((n, 1, d), (pitch, d, 1), d)
     k.copy_(randn(g, (n, 1, d), "fp16"))
     v.copy_(randn(g, (n, 1, d), "fp16"))
-    for nq in (1, 150):
+    for nq, algo in ((1, "mma"), (150, "mma"), (150, "tc")):
         q = randn(g, (nq, 1, d), "fp16", 3.0)
         out = torch.empty_like(q)
-        op = TokenAttention([0, nq], [0, n], 1, 1, d)
+        op = TokenAttention([0, nq], [0, n], 1, 1, d, algo=algo)
         op.run(ptr(q), ptr(k), ptr(v), ptr(out), k_strides=(pitch, d), v_strides=(pitch, d), stream=stream())
         ref, bound = attn_ref(q, k, v, [0, nq], [0, n], d ** -0.5)
         check(out, ref, bound, "fp16", "far offsets")
 
 
-def test_attention_nan_stays_in_its_document():
+@pytest.mark.parametrize("algo", ["mma", "tc"])
+def test_attention_nan_stays_in_its_document(algo):
     qs = [64, 70, 300, 1]
     off = np.cumsum([0] + qs)
     g = gen(19)
     q, k, v = (randn(g, (int(off[-1]), 2, 32), "fp16") for _ in range(3))
-    op = TokenAttention(off, off, 2, 2, 32)
+    op = TokenAttention(off, off, 2, 2, 32, algo=algo)
     a, b = torch.empty_like(q), torch.empty_like(q)
     op.run(ptr(q), ptr(k), ptr(v), ptr(a), stream=stream())
     k[off[1]:off[2]] = math.nan
@@ -389,9 +392,9 @@ def test_attention_nan_stays_in_its_document():
 
 def test_attention_repeats_bit_for_bit():
     g = gen(20)
-    for nq, nk in ((1, 9000), (500, 500), (64, 3000)):
+    for nq, nk, algo in ((1, 9000, "auto"), (500, 500, "tc"), (500, 500, "mma"), (64, 3000, "mma")):
         q, k, v = randn(g, (nq, 8, 64), "bf16"), randn(g, (nk, 2, 64), "bf16"), randn(g, (nk, 2, 64), "bf16")
-        op = TokenAttention([0, nq], [0, nk], 8, 2, 64, dtype="bf16")
+        op = TokenAttention([0, nq], [0, nk], 8, 2, 64, dtype="bf16", algo=algo)
         outs = []
         for _ in range(4):
             out = torch.empty_like(q)
@@ -400,9 +403,71 @@ def test_attention_repeats_bit_for_bit():
         assert all(torch.equal(outs[0], o) for o in outs[1:])
 
 
+@pytest.mark.parametrize("algo", ["mma", "tc"])
+@pytest.mark.parametrize("where", ["q", "k", "v"])
+def test_attention_infinities_and_nan_in_use_show(algo, where):
+    """A NaN or infinity that a row sees makes that row NaN or infinite, and no other row's query
+    is touched by one in q."""
+    for value in (math.nan, math.inf):
+        g = gen(24)
+        t = {n: randn(g, (200, 1, 64), "fp16") for n in ("q", "k", "v")}
+        t[where][77] = value
+        out = torch.zeros(200, 1, 64, dtype=torch.float16, device="cuda")
+        op = TokenAttention([0, 200], [0, 200], 1, 1, 64, algo=algo)
+        op.run(ptr(t["q"]), ptr(t["k"]), ptr(t["v"]), ptr(out), stream=stream())
+        bad = ~torch.isfinite(out).all(-1)[:, 0]
+        if where == "q":
+            assert bad.nonzero().flatten().tolist() == [77]
+        elif where == "v" or value != value:
+            assert bad.all()
+
+
 # ---------------------------------------------------------------------------
 # Graphs, streams, threads
 # ---------------------------------------------------------------------------
+FIRST_CALL_CAPTURED = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from arthip_b200.token_ops import AxisRotary, TokenAttention, TokenNorm
+x = torch.randn(200, 2, 64, device="cuda").half()
+outs = [torch.zeros_like(x) for _ in range(4)]
+pos = torch.zeros(1, 200, device="cuda")
+off = [0, 200]
+ops = [TokenNorm(128), AxisRotary(64, [64]), TokenAttention(off, off, 2, 2, 64, algo="mma"),
+       TokenAttention(off, off, 2, 2, 64, algo="tc")]
+p, o = x.data_ptr(), [t.data_ptr() for t in outs]
+def run(s):
+    ops[0].run(200, p, 0, o[0], stream=s)
+    ops[1].run(200, pos.data_ptr(), p, 2, o[1], stream=s)
+    ops[2].run(p, p, p, o[2], stream=s)
+    ops[3].run(p, p, p, o[3], stream=s)
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    run(side.cuda_stream)
+assert all((t == 0).all() for t in outs)
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in outs]
+run(torch.cuda.current_stream().cuda_stream)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and (a != 0).any() for a, b in zip(got, outs))
+print("captured first calls ok")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """Kernels load, and their attributes are set, on a first call: also under capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED.format(root=root)], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured first calls ok" in r.stdout, r.stderr[-2000:]
+
+
 def test_captured_run_follows_the_cache():
     """One graph, replayed while k_lens grows and after the inputs change."""
     d, cap_len = 64, 700
