@@ -8,8 +8,9 @@
 // never below the prefix. So a mask is two comparisons, made only in tiles that some row's
 // interval ends in, and tiles that no row sees are not loaded.
 //
-// Scores are kept as powers of two (x = score * log2 e), capped and biased in fp32. The weights 2^(x - max) are rounded to the tensors' type for the second product, as the
-// matrix instructions take no wider operand; their sum is taken before that rounding.
+// Scores are capped and biased in fp32. Their weights are rounded to the tensors' type for the
+// second product, as the matrix instructions take no wider operand; the sum of the weights is
+// taken before that rounding.
 //
 // Keys and values beyond a document's keys in use are filled with zeros as they are staged,
 // whatever the memory holds, so a NaN there cannot reach a sum through a weight of zero.
@@ -20,6 +21,7 @@
 // partial results are joined through distributed shared memory, so that no workspace is needed
 // and the order of the sums is fixed; and 64 rows with all their keys in one CTA, which takes
 // some key heads one after another, the next one's loads under way, and writes its rows itself.
+#include "ptx.cuh"
 #include "token_common.cuh"
 #include "tokens.h"
 
@@ -139,10 +141,14 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
   if (a.k_lens) klen = min(max(a.k_lens[item.doc], 0), doc.nk);
   const int rows = min(kRows, doc.nq * a.group - item.row0);
   const int prefix = min(doc.prefix, klen);
+  // A row's token within the document, and its head within the group. (Divisions by a number
+  // not known when compiling were a third of the instructions of a 64-token window.)
+  auto token_of = [&](int r) { return a.group == 1 ? item.row0 + r : (item.row0 + r) / a.group; };
+  auto member_of = [&](int r) { return a.group == 1 ? 0 : (item.row0 + r) % a.group; };
   // Row r sees the document's keys [0, hi(r)).
   auto hi_of = [&](int r) {
     if (!a.causal) return klen;
-    const int tok = (item.row0 + r) / a.group;
+    const int tok = token_of(r);
     return min(klen, max(prefix, klen - (doc.nq - tok) + 1));
   };
   const int hi_last = max(hi_of(rows - 1), 0);   // the largest
@@ -161,9 +167,9 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
     for (int i = threadIdx.x; i < kRows * kC; i += kThreads) {
       const int r = i / kC, c = i % kC;
       const bool take = r < rows && c < chunks;
-      const int row = item.row0 + (take ? r : 0);
-      const T* src = static_cast<const T*>(a.q) + (static_cast<long long>(doc.q0) + row / a.group) * a.q_tok +
-                     (kvh * a.group + row % a.group) * a.q_head + (take ? c * 8 : 0);
+      const int row = take ? r : 0;
+      const T* src = static_cast<const T*>(a.q) + (static_cast<long long>(doc.q0) + token_of(row)) * a.q_tok +
+                     (kvh * a.group + member_of(row)) * a.q_head + (take ? c * 8 : 0);
       cp_async16(sq + r * L::kRow + c * 16, src, take);
     }
   };
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
       float* sp = reinterpret_cast<float*>(st + L::kPos);
       for (int i = threadIdx.x; i < a.axes * kMmaKeys; i += kThreads) {
         const int ax = i / kMmaKeys, key = tile * kMmaKeys + i % kMmaKeys;
-        sp[i] = key < klen ? a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
+        sp[i] = key < klen ? -a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
       }
     }
   };
@@ -228,12 +234,12 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
     hi[e] = hi_of(r);
 #pragma unroll
     for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-      qpos[e][ax] = ax < a.axes ? a.q_pos[ax * a.q_total + doc.q0 + (item.row0 + r) / a.group] : 0.f;
+      qpos[e][ax] = ax < a.axes ? a.q_pos[ax * a.q_total + doc.q0 + token_of(r)] : 0.f;
   }
   auto load_slopes = [&](int kvh) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int h = kvh * a.group + (item.row0 + min(wrow + g + 8 * e, rows - 1)) % a.group;
+      const int h = kvh * a.group + member_of(min(wrow + g + 8 * e, rows - 1));
 #pragma unroll
       for (int ax = 0; ax < kAttnMaxAxes; ++ax) slope[e][ax] = ax < a.axes ? a.slopes[h * a.axes + ax] : 0.f;
     }
@@ -248,10 +254,9 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
   };
   reset();
   auto place = [&](int kvh, int r, int c) {  // of 8 elements of the output
-    const int row = item.row0 + r;
     return reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
-                                    (static_cast<long long>(doc.q0) + row / a.group) * a.o_tok +
-                                    (kvh * a.group + row % a.group) * a.o_head + c * 8);
+                                    (static_cast<long long>(doc.q0) + token_of(r)) * a.o_tok +
+                                    (kvh * a.group + member_of(r)) * a.o_head + c * 8);
   };
   auto join_lanes = [&] {
 #pragma unroll
@@ -266,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
     return;
   }
 
+  const float mul = a.cap_log2 > 0.f ? 1.f : a.score_mul;  // from the scores' units to powers of two
   uint32_t qf[kKD][4];
   int tile = tile0;
   for (int step = 0; step < steps; ++step) {
@@ -310,11 +316,6 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = attn_capped<kCapExp>(s[n][e], a);
-    } else {
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] *= a.score_mul;
     }
     if (a.axes) {
 #pragma unroll
@@ -322,11 +323,16 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
         if (ax >= a.axes) break;
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
-          const float2 kp = *reinterpret_cast<const float2*>(sp + ax * kMmaKeys + wk0 + n * 8 + t4 * 2);
-          s[n][0] -= slope[0][ax] * fabsf(qpos[0][ax] - kp.x);
-          s[n][1] -= slope[0][ax] * fabsf(qpos[0][ax] - kp.y);
-          s[n][2] -= slope[1][ax] * fabsf(qpos[1][ax] - kp.x);
-          s[n][3] -= slope[1][ax] * fabsf(qpos[1][ax] - kp.y);
+          const uint64_t away = *reinterpret_cast<const uint64_t*>(sp + ax * kMmaKeys + wk0 + n * 8 + t4 * 2);  // negated
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 far = ptx::unpack_f2(ptx::add_f2(ptx::pack_f2(qpos[e][ax], qpos[e][ax]), away));
+            const float2 z =
+                ptx::unpack_f2(ptx::fma_f2(ptx::pack_f2(fabsf(far.x), fabsf(far.y)),
+                                           ptx::pack_f2(-slope[e][ax], -slope[e][ax]),
+                                           ptx::pack_f2(s[n][2 * e], s[n][2 * e + 1])));
+            s[n][2 * e] = z.x, s[n][2 * e + 1] = z.y;
+          }
         }
       }
     }
@@ -342,20 +348,25 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
     for (int e = 0; e < 2; ++e) {
       float top = m[e];
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(s[n][2 * e], s[n][2 * e + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float base = top == -INFINITY ? 0.f : top;  // a row that has seen nothing yet
-      const float shrink = exp2_fast(m[e] - base), lift = base - kWeightShift;
+      for (int n = 0; n < kNT; ++n) top = ptx::max3_nan(top, s[n][2 * e], s[n][2 * e + 1]);
+      top = ptx::max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = ptx::max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // A row that has seen nothing yet weighs nothing; an infinite score makes a NaN, as the
+      // formula does.
+      const float base = top == -INFINITY ? 0.f : top;
+      const float shrink = exp2_fast((m[e] - base) * mul), lift = kWeightShift - base * mul;
       m[e] = top;
-      float sum = 0.f;
+      const uint64_t mul2 = ptx::pack_f2(mul, mul), lift2 = ptx::pack_f2(lift, lift);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
-        const float p0 = exp2_fast(s[n][2 * e] - lift), p1 = exp2_fast(s[n][2 * e + 1] - lift);
-        sum += p0 + p1;
+        const float2 x = ptx::unpack_f2(ptx::fma_f2(ptx::pack_f2(s[n][2 * e], s[n][2 * e + 1]), mul2, lift2));
+        const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
+        sum[n & 1] = ptx::add_f2(sum[n & 1], ptx::pack_f2(p0, p1));
         pf[n][e] = pack2<T>(p0, p1);
       }
-      l[e] = l[e] * shrink + sum;
+      const float2 total = ptx::unpack_f2(ptx::add_f2(sum[0], sum[1]));
+      l[e] = l[e] * shrink + (total.x + total.y);
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i) {
         o[i][2 * e] *= shrink;
@@ -390,9 +401,9 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
               pack2<T>(o[i][2 * e] * inv, o[i][2 * e + 1] * inv);
       }
       __syncwarp();
-      for (int i = lane; i < 16 * chunks; i += 32) {
-        const int r = wrow + i / chunks, c = i % chunks;
-        if (r < rows) *place(h, r, c) = *reinterpret_cast<const uint4*>(st + L::kStageQ + r * L::kRow + c * 16);
+      for (int i = lane; i < 16 * (DP / 8); i += 32) {
+        const int r = wrow + i / (DP / 8), c = i % (DP / 8);
+        if (r < rows && c < chunks) *place(h, r, c) = *reinterpret_cast<const uint4*>(st + L::kStageQ + r * L::kRow + c * 16);
       }
       tile = tile0;
       if (step + 1 < steps) {
@@ -439,14 +450,14 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
       if (i >= 16 * (DP / 8)) continue;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * 16 + r].x);
+      for (int w = 0; w < 4; ++w) top = ptx::max_nan(top, ml[w * 16 + r].x);
       mj[p] = make_float2(top, 0.f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[p][j] = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 v = ml[w * 16 + r];
-        const float k = v.x == -INFINITY ? 0.f : exp2_fast(v.x - top);
+        const float k = v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * mul);
         mj[p].y += k * v.y;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[p][j] += k * part[(w * 16 + r) * L::kPartRow + c * 8 + j];
@@ -473,10 +484,10 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
     float f[8], sum = 0.f, top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    for (int w = 0; w < ranks; ++w) top = fmaxf(top, cluster.map_shared_rank(ml, w)[r].x);
+    for (int w = 0; w < ranks; ++w) top = ptx::max_nan(top, cluster.map_shared_rank(ml, w)[r].x);
     for (int w = 0; w < ranks; ++w) {
       const float2 v = cluster.map_shared_rank(ml, w)[r];
-      const float k = v.x == -INFINITY ? 0.f : exp2_fast(v.x - top);
+      const float k = v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * mul);
       const float4* src =
           reinterpret_cast<const float4*>(cluster.map_shared_rank(part, w) + r * L::kPartRow + c * 8);
       const float4 x = src[0], y = src[1];

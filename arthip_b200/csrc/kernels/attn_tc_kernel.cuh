@@ -360,19 +360,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       for (int ax = t >> 7; ax < a.axes; ax += 2)
         put[ax * kTcKeys + (t & 127)] = key < klen ? -a.k_pos[ax * a.k_total + doc.k0 + key] : 0.f;
     };
-    const float mul = CAP || BIAS ? 1.f : a.score_mul;
+    const float mul = CAP ? 1.f : a.score_mul;  // from the scores' units to powers of two
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2];
     // Caps, biases and masks 64 columns of tile j and takes the rows' largest into `top`.
     auto prepare = [&](int j, int c, uint32_t(&x)[32], bool masked) {
       if constexpr (CAP || BIAS) {
+        if constexpr (CAP != kCapNone) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float v = __uint_as_float(x[e]);
-          if constexpr (CAP != kCapNone)
-            v = attn_capped<CAP>(v, a);
-          else
-            v *= a.score_mul;
-          x[e] = __float_as_uint(v);
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(attn_capped<CAP>(__uint_as_float(x[e]), a));
         }
         if constexpr (BIAS) {
           const float* pos = poss + (j & 1) * kAttnMaxAxes * kTcKeys + c * 64 + 2 * t4;

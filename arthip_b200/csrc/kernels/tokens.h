@@ -101,13 +101,13 @@ struct AttnArgs {
   const int* k_lens = nullptr;  // keys in use of each document, or null
   const AttnDoc* docs = nullptr;
   const AttnItem* items = nullptr;
-  const float* slopes = nullptr;  // [q heads][axes], times log2(e)
+  const float* slopes = nullptr;  // [q heads][axes], in the scores' units
   uint32_t* status = nullptr;
   int num_items = 0, num_sms = 148;
   int heads_per_block = 1;  // set by the launch that uses it
   int q_heads = 0, kv_heads = 0, group = 1, head_dim = 0, axes = 0, causal = 0;
-  // Scores in powers of two: x = score_mul * (q.k), or with a cap
-  // x = cap_log2 * tanh(cap_arg * (q.k)), with cap_exp = 2 log2(e) cap_arg.
+  // Scores: q.k less the bias, and times score_mul in powers of two; or with a cap, in powers of
+  // two before the bias, cap_log2 * tanh(cap_arg * (q.k)), with cap_exp = 2 log2(e) cap_arg.
   float score_mul = 0.f, cap_log2 = 0.f, cap_arg = 0.f, cap_exp = 0.f;
 };
 

@@ -480,9 +480,11 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   }
   const double kLog2e = 1.44269504088896340736;
   std::vector<float> bias(slopes ? static_cast<size_t>(d->q_heads) * d->axes : 0);
+  // In the units of the kernels' scores: powers of two behind a cap, else as the product q.k.
   for (size_t i = 0; i < bias.size(); ++i) {
-    if (!std::isfinite(slopes[i])) return Fail("attention: slopes must be finite", err, errlen);
-    bias[i] = static_cast<float>(slopes[i] * kLog2e);
+    bias[i] = static_cast<float>(d->cap > 0.f ? slopes[i] * kLog2e : static_cast<double>(slopes[i]) / d->scale);
+    if (!std::isfinite(slopes[i]) || !std::isfinite(bias[i]))
+      return Fail("attention: slopes, and slopes / scale, must be finite", err, errlen);
   }
   DeviceScope scope(device);
   auto h = std::make_unique<ah_attn>();
