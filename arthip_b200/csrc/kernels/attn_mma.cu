@@ -310,12 +310,18 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped<kCapSeries>(s[n][e], a);
+        for (int e = 0; e < 4; e += 2) {
+          const float2 v = ptx::unpack_f2(attn_capped2<kCapSeries>(ptx::pack_f2(s[n][e], s[n][e + 1]), a));
+          s[n][e] = v.x, s[n][e + 1] = v.y;
+        }
     } else if (a.cap_log2 > 0.f) {
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = attn_capped<kCapExp>(s[n][e], a);
+        for (int e = 0; e < 4; e += 2) {
+          const float2 v = ptx::unpack_f2(attn_capped2<kCapExp>(ptx::pack_f2(s[n][e], s[n][e + 1]), a));
+          s[n][e] = v.x, s[n][e + 1] = v.y;
+        }
     }
     if (a.axes) {
 #pragma unroll

@@ -367,7 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if constexpr (CAP || BIAS) {
         if constexpr (CAP != kCapNone) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(attn_capped<CAP>(__uint_as_float(x[e]), a));
+          for (int e = 0; e < 32; e += 2) {
+            const float2 v = ptx::unpack_f2(
+                attn_capped2<CAP>(ptx::pack_f2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a));
+            x[e] = __float_as_uint(v.x), x[e + 1] = __float_as_uint(v.y);
+          }
         }
         if constexpr (BIAS) {
           const float* pos = poss + (j & 1) * kAttnMaxAxes * kTcKeys + c * 64 + 2 * t4;

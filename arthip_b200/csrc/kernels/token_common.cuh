@@ -1,6 +1,7 @@
 // What the token kernels share: the capped score of attention, and launch attributes.
 #pragma once
 
+#include "ptx.cuh"
 #include "tokens.h"
 
 #include <atomic>
@@ -26,17 +27,26 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
+// Of two scores.
 template <int FORM>
-__device__ __forceinline__ float attn_capped(float s, const AttnArgs& a) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(s * a.cap_exp));
-  const float x = a.cap_log2 - 2.f * a.cap_log2 * rcp_fast(1.f + e);
+__device__ __forceinline__ uint64_t attn_capped2(uint64_t s, const AttnArgs& a) {
+  auto both = [](float v) { return ptx::pack_f2(v, v); };
+  float2 e = ptx::unpack_f2(ptx::mul_f2(s, both(a.cap_exp)));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+  const float2 d = ptx::unpack_f2(ptx::add_f2(ptx::pack_f2(e.x, e.y), both(1.f)));
+  const uint64_t x =
+      ptx::fma_f2(ptx::pack_f2(rcp_fast(d.x), rcp_fast(d.y)), both(-2.f * a.cap_log2), both(a.cap_log2));
   if constexpr (FORM == kCapSeries) {
     // tanh u = u - u^3/3 + 2u^5/15 - 17u^7/315 + 62u^9/2835; the next term is below 2^-24 u
-    const float u = s * a.cap_arg, z = u * u;
-    const float t =
-        a.cap_log2 * u * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835)))));
-    return fabsf(u) < 0.3f ? t : x;
+    const float2 sv = ptx::unpack_f2(s), xv = ptx::unpack_f2(x);
+    auto one = [&](float v, float big) {
+      const float u = v * a.cap_arg, z = u * u;
+      const float t =
+          a.cap_log2 * u * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835)))));
+      return fabsf(u) < 0.3f ? t : big;
+    };
+    return ptx::pack_f2(one(sv.x, xv.x), one(sv.y, xv.y));
   }
   return x;
 }

@@ -184,7 +184,7 @@ __device__ __forceinline__ float (&part(float (&f)[E], int n))[V] {
 // instead, 1280 channels ran at 60% of the copy rate, this way at 77%).
 template <typename T, int kV, int L, int N, int THREADS>
 __global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row_warps) {
-  extern __shared__ __align__(16) uint8_t smem[];  // [2 rows][x, y][N][threads] vectors
+  extern __shared__ __align__(16) uint8_t smem[];  // [2 rows][x, y, per-token gate][N][threads] vectors
   __shared__ float red_all[32];
   const int lanes = L ? L : row_warps * 32;
   const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
@@ -207,8 +207,10 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row
     load_weight<kV>(a.w, in[0] ? lane * kV : 0, 1.f, kw);
   }
 
+  const bool row_gate = gate && a.rows_per_gate == 1;
+  const int streams = row_gate ? 3 : 2;
   auto place = [&](int buf, int stream, int n) {
-    return reinterpret_cast<Vec<T, kV>*>(smem) + ((buf * 2 + stream) * N + n) * THREADS + threadIdx.x;
+    return reinterpret_cast<Vec<T, kV>*>(smem) + ((buf * streams + stream) * N + n) * THREADS + threadIdx.x;
   };
   auto fetch = [&](long long row, int buf) {
 #pragma unroll
@@ -217,6 +219,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row
       if (!in[n]) continue;
       copy_async<kV * 2>(place(buf, 0, n), x + row * a.xs + c);
       if (y) copy_async<kV * 2>(place(buf, 1, n), y + row * a.ys + c);
+      if (row_gate) copy_async<kV * 2>(place(buf, 2, n), gate + row * a.gs + c);
     }
   };
   // All lanes of a warp take as many steps as its first group, for the shuffles: a group
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row
     }
     if (y) {
       const T* grow = nullptr;
-      if (gate && live) grow = gate + (a.rows_per_gate == 1 ? row : row / a.rows_per_gate) * a.gs;
+      if (gate && !row_gate && live) grow = gate + row / a.rows_per_gate * a.gs;
       statistics<L, N * kV>(r, held, a.post, a.post_eps, inv_c, red, row_warps, bar, &mul, &add);
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -258,9 +261,9 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const NormArgs a, int row
 #pragma unroll
           for (int i = 0; i < kV; ++i) f[i] += kb[i];
         }
-        if (grow) {
+        if (grow || row_gate) {
           float g[kV];
-          unpack<T, kV>(load<T, kV>(grow + c), g);
+          unpack<T, kV>(row_gate ? *place(buf, 2, n) : load<T, kV>(grow + c), g);
           if (a.act != kGateLinear) {
 #pragma unroll
             for (int i = 0; i < kV; ++i) g[i] = gate_act(g[i], a.act);
@@ -327,16 +330,18 @@ cudaError_t resident_blocks(F fn, int threads, size_t smem, int num_sms, std::at
 template <typename T, int kV, int L, int N, int THREADS>
 cudaError_t launch(const NormArgs& a, int row_warps, int num_sms, cudaStream_t s) {
   auto fn = norm_kernel<T, kV, L, N, THREADS>;
-  static std::atomic<int> known[33];  // by row_warps
+  static std::atomic<int> known[32];  // by row_warps (at most 8), and 16 on with a per-token gate
   const int groups = THREADS / (L ? L : row_warps * 32);
   long long most;
-  constexpr int kSmem = 4 * N * THREADS * kV * 2;
+  const bool row_gate = a.gate && a.rows_per_gate == 1;
+  constexpr int kStream = 2 * N * THREADS * kV * 2;
+  const int smem = (row_gate ? 3 : 2) * kStream;
   static AttrOnce once;
-  cudaError_t e = once.set(reinterpret_cast<const void*>(fn), kSmem);
-  if (e == cudaSuccess) e = resident_blocks(fn, THREADS, kSmem, num_sms, known + row_warps, &most);
+  cudaError_t e = once.set(reinterpret_cast<const void*>(fn), 3 * kStream);
+  if (e == cudaSuccess) e = resident_blocks(fn, THREADS, smem, num_sms, known + row_warps + 16 * row_gate, &most);
   if (e != cudaSuccess) return e;
   const long long blocks = std::min<long long>((a.rows + groups - 1) / groups, most);
-  fn<<<static_cast<unsigned>(blocks), THREADS, kSmem, s>>>(a, row_warps);
+  fn<<<static_cast<unsigned>(blocks), THREADS, smem, s>>>(a, row_warps);
   return cudaGetLastError();
 }
 

@@ -6,9 +6,9 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <limits>
 #include <memory>
-#include <new>
 #include <string>
 #include <vector>
 
@@ -281,11 +281,11 @@ int ah_norm_create(int device, const ah_norm_desc* d, const float* post_weight, 
   h->args.wb = h->wb.as<float>();
   *out = h.release();
   return 0;
-} catch (const std::bad_alloc&) {
-  return Fail("norm: out of host memory", err, errlen);
+} catch (const std::exception& e) {
+  return Fail(std::string("norm: ") + e.what(), err, errlen);
 }
 
-int ah_norm_run(ah_norm* h, const ah_norm_io* io, void* stream, char* err, int errlen) {
+int ah_norm_run(ah_norm* h, const ah_norm_io* io, void* stream, char* err, int errlen) try {
   if (!h || !io) return Fail("invalid norm run arguments", err, errlen);
   if (io->rows < 0 || io->rows_per_gate < 1 || io->rows_per_mod < 1)
     return Fail("norm: rows must not be negative, rows_per_gate and rows_per_mod at least 1", err, errlen);
@@ -323,6 +323,8 @@ int ah_norm_run(ah_norm* h, const ah_norm_io* io, void* stream, char* err, int e
   a.rows = rows, a.rows_per_gate = io->rows_per_gate, a.rows_per_mod = io->rows_per_mod;
   const cudaError_t e = ah::norm_launch(a, h->dtype, h->num_sms, s);
   return e == cudaSuccess ? 0 : CudaFail("norm launch failed", e, err, errlen, 2);
+} catch (const std::exception& e) {
+  return Fail(std::string("norm: ") + e.what(), err, errlen, 2);
 }
 
 void ah_norm_destroy(ah_norm* h) {
@@ -386,12 +388,12 @@ int ah_rope_create(int device, const ah_rope_desc* d, ah_rope** out, char* err, 
   t.halves8 = halves8;
   *out = h.release();
   return 0;
-} catch (const std::bad_alloc&) {
-  return Fail("rope: out of host memory", err, errlen);
+} catch (const std::exception& e) {
+  return Fail(std::string("rope: ") + e.what(), err, errlen);
 }
 
 int ah_rope_run(ah_rope* h, int64_t tokens, const float* positions, const ah_rope_io* q, const ah_rope_io* k,
-                void* stream, char* err, int errlen) {
+                void* stream, char* err, int errlen) try {
   if (!h || !positions || (!q && !k)) return Fail("invalid rope run arguments", err, errlen);
   if (tokens < 0 || tokens > (int64_t(1) << 31) - 1) return Fail("rope: tokens must be 0..2^31-1", err, errlen);
   if (!Aligned(positions, 4)) return Fail("rope: positions must be 4-byte aligned", err, errlen);
@@ -430,6 +432,8 @@ int ah_rope_run(ah_rope* h, int64_t tokens, const float* positions, const ah_rop
   if (const int rc = CheckStream(s, h->device, err, errlen)) return rc;
   const cudaError_t e = ah::rope_launch(h->table, a, h->dtype, h->num_sms, s);
   return e == cudaSuccess ? 0 : CudaFail("rope launch failed", e, err, errlen, 2);
+} catch (const std::exception& e) {
+  return Fail(std::string("rope: ") + e.what(), err, errlen, 2);
 }
 
 void ah_rope_destroy(ah_rope* h) {
@@ -451,7 +455,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
                 errlen);
   if (d->kv_heads < 1 || d->kv_heads > 1024 || d->q_heads < 1 || d->q_heads > 1024 || d->q_heads % d->kv_heads)
     return Fail("attention: q_heads must be a multiple of kv_heads, both 1..1024", err, errlen);
-  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+  if (!(d->scale > 0.f) || !std::isfinite(2.f * d->scale))
     return Fail("attention: scale must be positive and finite", err, errlen);
   if (!(d->cap >= 0.f) || !std::isfinite(d->cap))
     return Fail("attention: cap must be finite, 0 for none", err, errlen);
@@ -556,11 +560,11 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   a.status = h->status.as<uint32_t>();
   *out = h.release();
   return 0;
-} catch (const std::bad_alloc&) {
-  return Fail("attention: out of host memory", err, errlen);
+} catch (const std::exception& e) {
+  return Fail(std::string("attention: ") + e.what(), err, errlen);
 }
 
-int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int errlen) {
+int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int errlen) try {
   if (!h || !io) return Fail("invalid attention run arguments", err, errlen);
   const int64_t D = h->args.head_dim, hq = h->args.q_heads, hk = h->args.kv_heads;
   auto view = [&](const void* p, int64_t tokens, int64_t tok, int64_t heads, int64_t head) {
@@ -615,6 +619,8 @@ int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int e
     e = ah::attn_mma_launch(a, h->dtype, true, h->few_cluster, h->few_tiles, s);
   }
   return e == cudaSuccess ? 0 : CudaFail(what.c_str(), e, err, errlen, 2);
+} catch (const std::exception& e) {
+  return Fail(std::string("attention: ") + e.what(), err, errlen, 2);
 }
 
 int ah_attn_status(ah_attn* h, uint32_t* status) {
