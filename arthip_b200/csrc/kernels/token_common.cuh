@@ -1,4 +1,5 @@
-// What the token kernels share: the capped score of attention, and launch attributes.
+// What the token kernels share: the capped score of attention, asynchronous copies of vectors and
+// of rows of any alignment, and launch attributes.
 #pragma once
 
 #include "ptx.cuh"
@@ -49,6 +50,50 @@ __device__ __forceinline__ uint64_t attn_capped2(uint64_t s, const AttnArgs& a) 
     return ptx::pack_f2(one(sv.x, xv.x), one(sv.y, xv.y));
   }
   return x;
+}
+
+// Asynchronous copies of a vector into shared memory, and their groups.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows of 2-byte elements between global memory and shared memory, by a group of GROUP threads,
+// in 16-byte pieces whatever their alignment; the elements before the first and behind the last
+// 16-byte boundary go one by one.
+// Elements [0, n) of `src` to where `dst` + (src % 16 bytes) starts. Waits for nothing.
+template <typename T, int GROUP>
+__device__ __forceinline__ void copy_in(uint8_t* dst, const T* src, int n, int t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(src);
+  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
+  T* d = reinterpret_cast<T*>(dst + at % 16);
+  if (t < head) d[t] = src[t];
+  for (int i = t; i < body; i += GROUP)
+    copy_async<16>(d + head + 8 * i, src + head + 8 * i);
+  const int tail = head + body * 8 + t;
+  if (tail < n) d[tail] = src[tail];
+}
+
+// The way back: elements [0, n) from `src` + (dst % 16 bytes).
+template <typename T, int GROUP>
+__device__ __forceinline__ void copy_out(T* dst, const uint8_t* src, int n, int t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
+  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
+  const T* from = reinterpret_cast<const T*>(src + at % 16);
+  if (t < head) dst[t] = from[t];
+  for (int i = t; i < body; i += GROUP)
+    *reinterpret_cast<uint4*>(dst + head + 8 * i) = *reinterpret_cast<const uint4*>(from + head + 8 * i);
+  const int tail = head + body * 8 + t;
+  if (tail < n) dst[tail] = from[tail];
 }
 
 // A kernel's function attributes, set once per device.

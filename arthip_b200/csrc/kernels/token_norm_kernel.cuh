@@ -157,20 +157,6 @@ __device__ __forceinline__ void statistics(const float (&f)[E], In in, int kind,
 // ---------------------------------------------------------------------------
 // Rows of vectors of 16, 8 or 4 bytes
 // ---------------------------------------------------------------------------
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 template <int V, int E>
 __device__ __forceinline__ float (&part(float (&f)[E], int n))[V] {
   return *reinterpret_cast<float(*)[V]>(f + n * V);
@@ -394,35 +380,6 @@ __device__ __forceinline__ void group_sync() {
     asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / GROUP), "n"(GROUP) : "memory");
 }
 
-// Elements [0, n) of `src` to where `dst` + (src % 16 bytes) starts. Waits for nothing.
-template <typename T, int GROUP>
-__device__ __forceinline__ void copy_in(uint8_t* dst, const T* src, int n, int t) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(src);
-  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
-  T* d = reinterpret_cast<T*>(dst + at % 16);
-  if (t < head) d[t] = src[t];
-  for (int i = t; i < body; i += GROUP)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                     static_cast<uint32_t>(__cvta_generic_to_shared(d + head + 8 * i))),
-                 "l"(src + head + 8 * i)
-                 : "memory");
-  const int tail = head + body * 8 + t;
-  if (tail < n) d[tail] = src[tail];
-}
-
-// The way back: elements [0, n) from `src` + (dst % 16 bytes).
-template <typename T, int GROUP>
-__device__ __forceinline__ void copy_out(T* dst, const uint8_t* src, int n, int t) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
-  const int head = min(n, static_cast<int>((16 - at % 16) % 16 / 2)), body = (n - head) / 8;
-  const T* from = reinterpret_cast<const T*>(src + at % 16);
-  if (t < head) dst[t] = from[t];
-  for (int i = t; i < body; i += GROUP)
-    *reinterpret_cast<uint4*>(dst + head + 8 * i) = *reinterpret_cast<const uint4*>(from + head + 8 * i);
-  const int tail = head + body * 8 + t;
-  if (tail < n) dst[tail] = from[tail];
-}
-
 struct Tiles {
   int rows = 1;         // of a tile
   int slot = 0;         // bytes of one stream's tile in shared memory
@@ -472,11 +429,11 @@ __global__ void __launch_bounds__(256, N <= 8 ? 3 : (N <= 16 ? 2 : 1)) norm_stag
   const long long step = static_cast<long long>(gridDim.x) * groups;
   long long tile = static_cast<long long>(blockIdx.x) * groups + group;
   if (tile < tiles.count) fetch(tile, 0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  copies_commit();
   for (int buf = 0; tile < tiles.count; tile += step, buf ^= 1) {
     if (tile + step < tiles.count) fetch(tile + step, buf ^ 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    copies_commit();
+    copies_wait<1>();
     group_sync<GROUP>();
     const uint8_t* from = base + buf * tiles.streams * tiles.slot;
     const long long row0 = tile * tiles.rows;

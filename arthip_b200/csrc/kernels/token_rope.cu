@@ -49,9 +49,17 @@ struct Two<__nv_bfloat16> {
 // How a head is cut into the units that one thread turns:
 //   kUnitPairs   8 elements, four adjacent pairs
 //   kUnitHalves  8 pairs: 8 elements and the 8 elements that turn with them
-//   kUnitOne     one pair, element by element
-// Elements behind the rotated part are copied, 8 (or 1) at a time.
-enum Unit : int { kUnitPairs = 0, kUnitHalves = 1, kUnitOne = 2 };
+// Elements behind the rotated part are copied, 8 at a time. Heads that cannot be cut so have a
+// kernel of their own, below.
+enum Unit : int { kUnitPairs = 0, kUnitHalves = 1 };
+
+// Cosine and sine of a pair at a token's position.
+__device__ __forceinline__ float2 turn_of(const RopePair& p, const RopeArgs& a, long long tok) {
+  const double turns = static_cast<double>(a.pos[p.axis * a.tokens + tok]) * p.turns;
+  float s, c;
+  sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+  return make_float2(c, s);
+}
 
 // How a block's threads are laid out over a pass: `width` places of a head, `heads` heads,
 // `tokens` tokens.
@@ -66,10 +74,10 @@ constexpr int kRopeDepth = 4;  // items of a thread in flight
 template <typename T, int UNIT>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeTable t, const RopeArgs a, const RopeGrid g) {
   constexpr int kVecs = UNIT == kUnitHalves ? 2 : 1;  // 16-byte vectors of an item
-  constexpr int kPairs = UNIT == kUnitPairs ? 4 : (UNIT == kUnitHalves ? 8 : 1);
+  constexpr int kPairs = UNIT == kUnitPairs ? 4 : 8;
   extern __shared__ __align__(16) uint8_t smem[];
   uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;  // [depth][vector][thread]
-  float2* cs = reinterpret_cast<float2*>(smem + (UNIT == kUnitOne ? 0 : kRopeDepth * kVecs * kRopeThreads * 16));
+  float2* cs = reinterpret_cast<float2*>(smem + kRopeDepth * kVecs * kRopeThreads * 16);
   using T2 = typename Two<T>::type;
   const long long tok0 = static_cast<long long>(blockIdx.x) * g.tok_per_block;
   const int ntok = static_cast<int>(min(static_cast<long long>(g.tok_per_block), a.tokens - tok0));
@@ -104,76 +112,48 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeTable t, c
       const T* in = source(next_tok, next_h);
 #pragma unroll
       for (int v = 0; v < kVecs; ++v)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
-                         __cvta_generic_to_shared(ring + (at * kVecs + v) * kRopeThreads))),
-                     "l"(in + (v ? e1 : e0))
-                     : "memory");
+        copy_async<16>(ring + (at * kVecs + v) * kRopeThreads, in + (v ? e1 : e0));
       advance(&next_tok, &next_h);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    copies_commit();
   };
-  if constexpr (UNIT != kUnitOne) {
 #pragma unroll
-    for (int d = 0; d < kRopeDepth; ++d) issue(d);
-  }
+  for (int d = 0; d < kRopeDepth; ++d) issue(d);
   for (int i = threadIdx.x; i < ntok * t.npairs; i += kRopeThreads) {
     const int tok = i / t.npairs;
-    const RopePair p = t.pairs[i - tok * t.npairs];
-    const double turns = static_cast<double>(a.pos[p.axis * a.tokens + tok0 + tok]) * p.turns;
-    float s, c;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c, s);
+    cs[i] = turn_of(t.pairs[i - tok * t.npairs], a, tok0 + tok);
   }
   __syncthreads();
-  if constexpr (UNIT == kUnitOne) {  // heads whose parts are no vectors: element by element
-    for (int u = u0; u < g.units; u += g.width) {
-      const bool turns = u < g.turn_units;
-      const int i0 = turns ? t.pairs[u].e0 : t.rot + u - g.turn_units, i1 = turns ? t.pairs[u].e1 : i0;
-      for (int tok = first, h = h0; tok < ntok; advance(&tok, &h)) {
-        const T* in = source(tok, h);
-        T* out = target(tok, h);
-        if (!turns) {
-          out[i0] = in[i0];
-          continue;
-        }
-        const float2 c = cs[tok * t.npairs + u];
-        const float x = to_f(in[i0]), y = to_f(in[i1]);
-        from_f(x * c.x - y * c.y, out + i0);
-        from_f(x * c.y + y * c.x, out + i1);
+  float2 c[kPairs];
+  int have = -1;  // the token that c is of
+  for (int tok = first, h = h0, at = 0; tok < ntok; advance(&tok, &h), at = (at + 1) % kRopeDepth) {
+    copies_wait<kRopeDepth - 1>();
+    uint4 v[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) v[i] = ring[(at * kVecs + i) * kRopeThreads];
+    issue(at);
+    T* out = target(tok, h);
+    if (turn) {
+      if (tok != have) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) c[j] = cs[tok * t.npairs + u0 * kPairs + j];
+        have = tok;
       }
-    }
-  } else {
-    float2 c[kPairs];
-    int have = -1;  // the token that c is of
-    for (int tok = first, h = h0, at = 0; tok < ntok; advance(&tok, &h), at = (at + 1) % kRopeDepth) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRopeDepth - 1) : "memory");
-      uint4 v[kVecs];
+      T2* pa = reinterpret_cast<T2*>(v);
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) v[i] = ring[(at * kVecs + i) * kRopeThreads];
-      issue(at);
-      T* out = target(tok, h);
-      if (turn) {
-        if (tok != have) {
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) c[j] = cs[tok * t.npairs + u0 * kPairs + j];
-          have = tok;
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = unpack(pa[j]);
+        if constexpr (UNIT == kUnitPairs) {
+          pack(make_float2(x.x * c[j].x - x.y * c[j].y, x.x * c[j].y + x.y * c[j].x), pa + j);
+        } else {
+          const float2 c0 = c[2 * j], c1 = c[2 * j + 1], y = unpack(pa[4 + j]);
+          pack(make_float2(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y), pa + j);
+          pack(make_float2(x.x * c0.y + y.x * c0.x, x.y * c1.y + y.y * c1.x), pa + 4 + j);
         }
-        T2* pa = reinterpret_cast<T2*>(v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 x = unpack(pa[j]);
-          if constexpr (UNIT == kUnitPairs) {
-            pack(make_float2(x.x * c[j].x - x.y * c[j].y, x.x * c[j].y + x.y * c[j].x), pa + j);
-          } else {
-            const float2 c0 = c[2 * j], c1 = c[2 * j + 1], y = unpack(pa[4 + j]);
-            pack(make_float2(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y), pa + j);
-            pack(make_float2(x.x * c0.y + y.x * c0.x, x.y * c1.y + y.y * c1.x), pa + 4 + j);
-          }
-        }
-        if constexpr (UNIT == kUnitHalves) *reinterpret_cast<uint4*>(out + e1) = v[1];
       }
-      *reinterpret_cast<uint4*>(out + e0) = v[0];
+      if constexpr (UNIT == kUnitHalves) *reinterpret_cast<uint4*>(out + e1) = v[1];
     }
+    *reinterpret_cast<uint4*>(out + e0) = v[0];
   }
 }
 
@@ -181,8 +161,8 @@ template <typename T, int UNIT>
 cudaError_t launch(const RopeTable& t, const RopeArgs& a, int num_sms, cudaStream_t s) {
   const int tail = t.head_dim - t.rot, all = a.heads[0] + a.heads[1];
   RopeGrid g;
-  g.turn_units = UNIT == kUnitPairs ? t.rot / 8 : (UNIT == kUnitHalves ? t.npairs / 8 : t.npairs);
-  g.units = g.turn_units + (UNIT == kUnitOne ? tail : tail / 8);
+  g.turn_units = UNIT == kUnitPairs ? t.rot / 8 : t.npairs / 8;
+  g.units = g.turn_units + tail / 8;
   g.width = std::min(g.units, kRopeThreads);
   // Neighbouring threads on neighbouring heads, up to 1 KB of a token.
   g.heads = std::min({std::max(1, 64 / g.width), all, kRopeThreads / g.width});
@@ -194,12 +174,119 @@ cudaError_t launch(const RopeTable& t, const RopeArgs& a, int num_sms, cudaStrea
   g.tok_per_block = static_cast<int>(passes > 0 ? passes * g.tokens : std::clamp<long long>(spread, 1, most));
   const long long blocks = (a.tokens + g.tok_per_block - 1) / g.tok_per_block;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  constexpr int kRing = UNIT == kUnitOne ? 0 : kRopeDepth * (UNIT == kUnitHalves ? 2 : 1) * kRopeThreads * 16;
+  constexpr int kRing = kRopeDepth * (UNIT == kUnitHalves ? 2 : 1) * kRopeThreads * 16;
   auto fn = rope_kernel<T, UNIT>;
   static AttrOnce once;
   const cudaError_t e = once.set(reinterpret_cast<const void*>(fn), kRing + kRopeTableBytes + 4096);
   if (e != cudaSuccess) return e;
   fn<<<static_cast<unsigned>(blocks), kRopeThreads, kRing + g.tok_per_block * t.npairs * sizeof(float2), s>>>(t, a, g);
+  return cudaGetLastError();
+}
+
+// Heads of any cut, width, stride and alignment: a warp takes a run of a token's heads into shared
+// memory in 16-byte pieces, one run ahead, turns its pairs there and sends them out the same way.
+// A lane's pairs are every 32nd of a head, their cosines and sines in registers for all heads of
+// the token. (Turned in global memory, pair by pair, such heads ran at 31% of the copy rate.)
+struct RopeRuns {
+  int slot = 0;         // bytes of a run in shared memory
+  int heads[2] = {};    // of a run of q, of k
+  int runs[2] = {};     // of a token
+};
+
+template <typename T, int KP>
+__global__ void __launch_bounds__(kRopeThreads) rope_staged_kernel(const RopeTable t, const RopeArgs a,
+                                                                   const RopeRuns g) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kWarps = kRopeThreads / 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t* mine = smem + warp * 3 * g.slot;  // two runs on their way in, one on its way out
+  uint8_t* out_at = mine + 2 * g.slot;
+  const int per_tok = g.runs[0] + g.runs[1];
+  struct Run {
+    const T* in;
+    T* out;
+    long long in_step, out_step;  // between heads
+    int heads;
+  };
+  auto run_of = [&](long long tok, int r) {
+    const bool k = r >= g.runs[0];
+    const int each = k ? g.heads[1] : g.heads[0], h = (k ? r - g.runs[0] : r) * each;
+    Run x;
+    x.in_step = k ? a.in_head[1] : a.in_head[0], x.out_step = k ? a.out_head[1] : a.out_head[0];
+    x.in = static_cast<const T*>(k ? a.in[1] : a.in[0]) + tok * (k ? a.in_tok[1] : a.in_tok[0]) + h * x.in_step;
+    x.out = static_cast<T*>(k ? a.out[1] : a.out[0]) + tok * (k ? a.out_tok[1] : a.out_tok[0]) + h * x.out_step;
+    x.heads = min(each, (k ? a.heads[1] : a.heads[0]) - h);
+    return x;
+  };
+  int e0[KP], e1[KP];
+#pragma unroll
+  for (int k = 0; k < KP; ++k) {
+    const int p = min(lane + 32 * k, t.npairs - 1);
+    e0[k] = t.pairs[p].e0, e1[k] = t.pairs[p].e1;
+  }
+  const long long step = static_cast<long long>(gridDim.x) * kWarps;
+  long long tok = static_cast<long long>(blockIdx.x) * kWarps + warp, next_tok = tok;
+  int next_r = 0;
+  auto fetch = [&](int buf) {
+    if (next_tok < a.tokens) {
+      const Run x = run_of(next_tok, next_r);
+      copy_in<T, 32>(mine + buf * g.slot, x.in, x.heads * t.head_dim, lane);
+      if (++next_r == per_tok) next_r = 0, next_tok += step;
+    }
+    copies_commit();
+  };
+  fetch(0);
+  int buf = 0;
+  for (; tok < a.tokens; tok += step) {
+    float2 c[KP];
+#pragma unroll
+    for (int k = 0; k < KP; ++k) c[k] = turn_of(t.pairs[min(lane + 32 * k, t.npairs - 1)], a, tok);
+    for (int r = 0; r < per_tok; ++r, buf ^= 1) {
+      fetch(buf ^ 1);
+      copies_wait<1>();
+      __syncwarp();
+      const Run x = run_of(tok, r);
+      const T* from = reinterpret_cast<const T*>(mine + buf * g.slot + reinterpret_cast<uintptr_t>(x.in) % 16);
+      T* to = reinterpret_cast<T*>(out_at + reinterpret_cast<uintptr_t>(x.out) % 16);
+      for (int h = 0; h < x.heads; ++h, from += t.head_dim, to += t.head_dim) {
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+          if (lane + 32 * k >= t.npairs) continue;
+          const float u = to_f(from[e0[k]]), v = to_f(from[e1[k]]);
+          from_f(u * c[k].x - v * c[k].y, to + e0[k]);
+          from_f(u * c[k].y + v * c[k].x, to + e1[k]);
+        }
+        for (int e = t.rot + lane; e < t.head_dim; e += 32) to[e] = from[e];
+      }
+      __syncwarp();
+      copy_out<T, 32>(x.out, out_at, x.heads * t.head_dim, lane);
+      __syncwarp();  // the results have left, and this run's places may be written over
+    }
+  }
+}
+
+template <typename T, int KP>
+cudaError_t launch_staged(const RopeTable& t, const RopeArgs& a, int num_sms, cudaStream_t s) {
+  RopeRuns g;
+  int most = 0;
+  for (int w = 0; w < 2; ++w) {
+    if (a.heads[w] == 0) continue;
+    // Heads one behind the other make one run, up to 4 KB; others go one by one.
+    const bool packed = a.heads[w] == 1 || (a.in_head[w] == t.head_dim && a.out_head[w] == t.head_dim);
+    g.heads[w] = packed ? std::clamp(2048 / t.head_dim, 1, a.heads[w]) : 1;
+    g.runs[w] = (a.heads[w] + g.heads[w] - 1) / g.heads[w];
+    most = std::max(most, g.heads[w]);
+  }
+  g.slot = (most * t.head_dim * 2 + 15) / 16 * 16 + 16;
+  constexpr int kWarps = kRopeThreads / 32;
+  const int smem = kWarps * 3 * g.slot;
+  auto fn = rope_staged_kernel<T, KP>;
+  static AttrOnce once;
+  const cudaError_t e = once.set(reinterpret_cast<const void*>(fn), kWarps * 3 * (4096 + 32));
+  if (e != cudaSuccess) return e;
+  const long long places = static_cast<long long>(num_sms) * std::clamp(220 * 1024 / (smem + 1024), 1, 6);
+  const long long blocks = std::min<long long>((a.tokens + kWarps - 1) / kWarps, places);
+  fn<<<static_cast<unsigned>(blocks), kRopeThreads, smem, s>>>(t, a, g);
   return cudaGetLastError();
 }
 
@@ -217,7 +304,10 @@ cudaError_t by_unit(const RopeTable& t, const RopeArgs& a, int num_sms, cudaStre
     if (t.layout == kRopePairs) return launch<T, kUnitPairs>(t, a, num_sms, s);
     if (t.halves8) return launch<T, kUnitHalves>(t, a, num_sms, s);
   }
-  return launch<T, kUnitOne>(t, a, num_sms, s);
+  if (t.npairs <= 32) return launch_staged<T, 1>(t, a, num_sms, s);
+  if (t.npairs <= 64) return launch_staged<T, 2>(t, a, num_sms, s);
+  if (t.npairs <= 128) return launch_staged<T, 4>(t, a, num_sms, s);
+  return launch_staged<T, 8>(t, a, num_sms, s);
 }
 
 }  // namespace
