@@ -11,9 +11,10 @@
 // registers, so a large mean costs no digits.
 //
 // Bound: HBM, 8 bytes per element (y, x in; out, norm out), 10 with a per-token gate. Two
-// kernels: rows of whole vectors of 16, 8 or 4 bytes, and rows of any width, stride or
-// alignment, which pass through shared memory in 16-byte pieces all the same (loaded element by
-// element, 91 channels ran at 9% of the copy rate; this way at 40%).
+// kernels: rows of whole vectors of 16 or 8 bytes (2073600 rows of 64: 178 us, 93% of the copy
+// rate), and rows of any width, stride or alignment, which pass through shared memory in 16-byte
+// pieces all the same (64 Mi elements in rows of 91: loaded element by element 951 us, this way
+// 144 us, 58% of the copy rate, bound by the instructions per element).
 #pragma once
 
 #include "token_common.cuh"
@@ -155,7 +156,7 @@ __device__ __forceinline__ void statistics(const float (&f)[E], In in, int kind,
 }
 
 // ---------------------------------------------------------------------------
-// Rows of vectors of 16, 8 or 4 bytes
+// Rows of vectors of 16 or 8 bytes
 // ---------------------------------------------------------------------------
 template <int V, int E>
 __device__ __forceinline__ float (&part(float (&f)[E], int n))[V] {
@@ -355,9 +356,7 @@ cudaError_t by_width(const NormArgs& a, int num_sms, cudaStream_t s) {
   if (n <= 768) return launch<T, V, 0, 6, 128>(a, 4, num_sms, s);
   if (n <= 1024) return launch<T, V, 0, 4, 256>(a, 8, num_sms, s);
   // n is at most 8192 / V
-  if constexpr (V < 8)
-    if (n <= 2048) return launch<T, V, 0, 8, 256>(a, 8, num_sms, s);
-  if constexpr (V == 2) return launch<T, V, 0, 16, 256>(a, 8, num_sms, s);
+  if constexpr (V < 8) return launch<T, V, 0, 8, 256>(a, 8, num_sms, s);
   return cudaErrorInvalidValue;
 }
 
@@ -370,8 +369,7 @@ cudaError_t by_width(const NormArgs& a, int num_sms, cudaStream_t s) {
 // way. LANES lanes share a row (a warp has 32 / LANES at once), element e being lane e % LANES'.
 // A lane's N channels are the same in every row, and their weights stay in registers. N is even
 // and at most one more than a lane needs, so that only its last two elements are ever in
-// question: with a test for each (N in steps of 4 and 8), 90 channels took 85 instructions an
-// element and ran at 34% of the copy rate.
+// question (with a test for each, 90 channels took 85 instructions an element).
 template <int GROUP>
 __device__ __forceinline__ void group_sync() {
   if constexpr (GROUP == 32)
@@ -555,14 +553,15 @@ cudaError_t by_count(const NormArgs& a, int num_sms, cudaStream_t s) {
   return launch_staged<T, GROUP, LANES, LO>(a, num_sms, s);
 }
 
-// 5 to 16 elements a lane: a row's fixed work (the sums across lanes, the choices) is shared by
+// 9 to 16 elements a lane: a row's fixed work (the sums across lanes, the choices) is shared by
 // as many rows at once as that leaves lanes for.
 template <typename T>
 cudaError_t by_elements(const NormArgs& a, int num_sms, cudaStream_t s) {
   if (a.C <= 32) return by_count<T, 32, 4, 2, 8>(a, num_sms, s);
-  if (a.C <= 64) return by_count<T, 32, 8, 6, 8>(a, num_sms, s);
-  if (a.C <= 128) return by_count<T, 32, 16, 6, 8>(a, num_sms, s);
-  if (a.C <= 512) return by_count<T, 32, 32, 6, 16>(a, num_sms, s);
+  if (a.C <= 64) return by_count<T, 32, 4, 10, 16>(a, num_sms, s);
+  if (a.C <= 128) return by_count<T, 32, 8, 10, 16>(a, num_sms, s);
+  if (a.C <= 256) return by_count<T, 32, 16, 10, 16>(a, num_sms, s);
+  if (a.C <= 512) return by_count<T, 32, 32, 10, 16>(a, num_sms, s);
   if (a.C <= 1024) return by_count<T, 64, 64, 10, 16>(a, num_sms, s);
   if (a.C <= 2048) return by_count<T, 128, 128, 10, 16>(a, num_sms, s);
   if (a.C <= 4096) return by_count<T, 256, 256, 10, 16>(a, num_sms, s);

@@ -5,9 +5,7 @@ namespace ah {
 namespace token_norm {
 
 cudaError_t vectors_bf16(const NormArgs& a, int vec, int num_sms, cudaStream_t s) {
-  if (vec == 8) return by_width<__nv_bfloat16, 8>(a, num_sms, s);
-  if (vec == 4) return by_width<__nv_bfloat16, 4>(a, num_sms, s);
-  return by_width<__nv_bfloat16, 2>(a, num_sms, s);
+  return vec == 8 ? by_width<__nv_bfloat16, 8>(a, num_sms, s) : by_width<__nv_bfloat16, 4>(a, num_sms, s);
 }
 
 }  // namespace token_norm
