@@ -528,6 +528,30 @@ def test_one_handle_on_two_streams_and_threads():
     assert not errors and all(torch.equal(a, b) for a, b in zip(outs, wants))
 
 
+def test_two_graphs_of_one_handle_run_side_by_side():
+    """Split keys are joined without a workspace, so graphs of one handle share nothing."""
+    g = gen(25)
+    op = TokenAttention([0, 1], [0, 30000], 4, 2, 64)
+    sets = [[randn(g, (1, 4, 64), "fp16"), randn(g, (30000, 2, 64), "fp16"), randn(g, (30000, 2, 64), "fp16")]
+            for _ in range(2)]
+    outs, wants, graphs, streams = [], [], [], []
+    for q, k, v in sets:
+        want, out = torch.empty_like(q), torch.zeros_like(q)
+        op.run(ptr(q), ptr(k), ptr(v), ptr(want), stream=stream())
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            for _ in range(20):
+                op.run(ptr(q), ptr(k), ptr(v), ptr(out), stream=side.cuda_stream)
+        outs.append(out), wants.append(want), graphs.append(graph), streams.append(side)
+    for _ in range(5):
+        for graph, side in zip(graphs, streams):
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+
+
 def test_run_refusals_launch_nothing():
     q = torch.zeros(64, 2, 32, dtype=torch.float16, device="cuda")
     out = torch.full_like(q, 7.0)
