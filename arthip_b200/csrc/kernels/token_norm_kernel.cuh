@@ -18,6 +18,7 @@
 #pragma once
 
 #include "token_common.cuh"
+#include "token_norm_shape.h"
 #include "tokens.h"
 
 #include <algorithm>
@@ -368,8 +369,8 @@ cudaError_t by_width(const NormArgs& a, int num_sms, cudaStream_t s) {
 // before the first and behind the last 16-byte boundary one by one; the results leave the same
 // way. LANES lanes share a row (a warp has 32 / LANES at once), element e being lane e % LANES'.
 // A lane's N channels are the same in every row, and their weights stay in registers. N is even
-// and at most one more than a lane needs, so that only its last two elements are ever in
-// question (with a test for each, 90 channels took 85 instructions an element).
+// and at most one more than a lane needs (staged_shape), so that only its last two elements are
+// ever in question (with a test for each, 90 channels took 85 instructions an element).
 template <int GROUP>
 __device__ __forceinline__ void group_sync() {
   if constexpr (GROUP == 32)
@@ -545,27 +546,20 @@ cudaError_t launch_staged(const NormArgs& a, int num_sms, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// The launch with the N that C needs of [LO, HI] (even numbers), LANES lanes a row.
-template <typename T, int GROUP, int LANES, int LO, int HI>
-cudaError_t by_count(const NormArgs& a, int num_sms, cudaStream_t s) {
-  if constexpr (LO < HI)
-    if (a.C > LO * LANES) return by_count<T, GROUP, LANES, LO + 2, HI>(a, num_sms, s);
-  return launch_staged<T, GROUP, LANES, LO>(a, num_sms, s);
-}
+template <typename T>
+struct LaunchStaged {
+  const NormArgs& a;
+  int num_sms;
+  cudaStream_t s;
+  template <int GROUP, int LANES, int N>
+  cudaError_t operator()() const {
+    return launch_staged<T, GROUP, LANES, N>(a, num_sms, s);
+  }
+};
 
-// 9 to 16 elements a lane: a row's fixed work (the sums across lanes, the choices) is shared by
-// as many rows at once as that leaves lanes for.
 template <typename T>
 cudaError_t by_elements(const NormArgs& a, int num_sms, cudaStream_t s) {
-  if (a.C <= 32) return by_count<T, 32, 4, 2, 8>(a, num_sms, s);
-  if (a.C <= 64) return by_count<T, 32, 4, 10, 16>(a, num_sms, s);
-  if (a.C <= 128) return by_count<T, 32, 8, 10, 16>(a, num_sms, s);
-  if (a.C <= 256) return by_count<T, 32, 16, 10, 16>(a, num_sms, s);
-  if (a.C <= 512) return by_count<T, 32, 32, 10, 16>(a, num_sms, s);
-  if (a.C <= 1024) return by_count<T, 64, 64, 10, 16>(a, num_sms, s);
-  if (a.C <= 2048) return by_count<T, 128, 128, 10, 16>(a, num_sms, s);
-  if (a.C <= 4096) return by_count<T, 256, 256, 10, 16>(a, num_sms, s);
-  return by_count<T, 256, 256, 20, 32>(a, num_sms, s);
+  return staged_shape(a.C, LaunchStaged<T>{a, num_sms, s});
 }
 
 // One translation unit each (token_norm_*.cu): rows of vectors (of `vec` elements), any rows.
