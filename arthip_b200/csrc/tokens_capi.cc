@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <limits>
 #include <memory>
 #include <string>
@@ -74,6 +75,17 @@ class DeviceBuffer {
  private:
   void* p_ = nullptr;
 };
+
+// Waits for the uploads of a handle's buffers. A copy from pageable memory may return before it
+// has arrived, ordered with the legacy stream only, while the handle's first run may come at once
+// on a stream that does not wait for that one. A copy back is behind them, and done on return.
+cudaError_t AwaitUploads(std::initializer_list<const DeviceBuffer*> buffers) {
+  for (const DeviceBuffer* b : buffers) {
+    char byte;
+    if (b->as<char>()) return cudaMemcpy(&byte, b->as<char>(), 1, cudaMemcpyDeviceToHost);
+  }
+  return cudaSuccess;
+}
 
 int CheckDevice(const DeviceScope& scope, int device, int* num_sms, char* err, int errlen) {
   if (scope.error() != cudaSuccess) {
@@ -274,6 +286,7 @@ int ah_norm_create(int device, const ah_norm_desc* d, const float* post_weight, 
   }
   if (e == cudaSuccess && pre_weight) e = h->w.Upload(pre_weight, bytes);
   if (e == cudaSuccess && pre_bias) e = h->wb.Upload(pre_bias, bytes);
+  if (e == cudaSuccess) e = AwaitUploads({&h->a, &h->b, &h->w, &h->wb});
   if (e != cudaSuccess) return CudaFail("norm weight upload failed", e, err, errlen, 1);
   h->args.a = h->a.as<float>();
   h->args.b = h->b.as<float>();
@@ -376,7 +389,8 @@ int ah_rope_create(int device, const ah_rope_desc* d, ah_rope** out, char* err, 
       pairs.push_back(p);
     }
   }
-  const cudaError_t e = h->pairs.Upload(pairs.data(), pairs.size() * sizeof(ah::RopePair));
+  cudaError_t e = h->pairs.Upload(pairs.data(), pairs.size() * sizeof(ah::RopePair));
+  if (e == cudaSuccess) e = AwaitUploads({&h->pairs});
   if (e != cudaSuccess) return CudaFail("rope table upload failed", e, err, errlen, 1);
   ah::RopeTable& t = h->table;
   t.pairs = h->pairs.as<ah::RopePair>();
@@ -554,6 +568,7 @@ int ah_attn_create(int device, const ah_attn_desc* d, int docs, const int64_t* q
   if (e == cudaSuccess) e = h->slopes.Upload(bias.data(), bias.size() * sizeof(float));
   const uint32_t zero = 0;
   if (e == cudaSuccess) e = h->status.Upload(&zero, sizeof zero);
+  if (e == cudaSuccess) e = AwaitUploads({&h->status});
   if (e != cudaSuccess) return CudaFail("attention plan upload failed", e, err, errlen, 1);
   a.docs = h->docs.as<ah::AttnDoc>();
   a.slopes = h->slopes.as<float>();

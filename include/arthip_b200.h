@@ -209,8 +209,8 @@ int ah_conv3x3_run_noalloc(int device, int C, int M, const uint16_t* w_oihw_f16,
  * frame is [tokens][channels] as it stands. Element types: 0 = fp16, 1 = bf16. Sums,
  * statistics and softmax weights' sums are fp32.
  *
- * A handle holds uploaded parameters only and does not change after creation: runs of one
- * handle may overlap on any streams and threads and be captured into CUDA graphs. A run is
+ * A handle holds uploaded parameters only, has them on the device when its creation returns, and
+ * does not change after that: runs of one handle may overlap on any streams and threads and be captured into CUDA graphs. A run is
  * asynchronous on `stream` (cudaStream_t of the handle's device, NULL = legacy default),
  * allocates no device memory and leaves the caller's current device as it was. Tensors are in
  * memory of the handle's device. Strides count elements; 0 means packed. Inputs may be slices
