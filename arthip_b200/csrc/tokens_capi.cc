@@ -643,7 +643,10 @@ int ah_attn_status(ah_attn* h, uint32_t* status) {
   DeviceScope scope(h->device);
   if (scope.error() != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) return 2;
   if (cudaMemcpy(status, h->args.status, sizeof(uint32_t), cudaMemcpyDeviceToHost) != cudaSuccess) return 2;
-  return cudaMemset(h->args.status, 0, sizeof(uint32_t)) == cudaSuccess ? 0 : 2;
+  if (*status == 0) return 0;
+  // The fill is waited for, so that it cannot wipe out what a later run reports.
+  if (cudaMemset(h->args.status, 0, sizeof(uint32_t)) != cudaSuccess) return 2;
+  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
 }
 
 void ah_attn_destroy(ah_attn* h) {

@@ -210,12 +210,13 @@ int ah_conv3x3_run_noalloc(int device, int C, int M, const uint16_t* w_oihw_f16,
  * statistics and softmax weights' sums are fp32.
  *
  * A handle holds uploaded parameters only, has them on the device when its creation returns, and
- * does not change after that: runs of one handle may overlap on any streams and threads and be captured into CUDA graphs. A run is
- * asynchronous on `stream` (cudaStream_t of the handle's device, NULL = legacy default),
- * allocates no device memory and leaves the caller's current device as it was. Tensors are in
- * memory of the handle's device. Strides count elements; 0 means packed. Inputs may be slices
- * of one buffer. Return codes as above; a run that returns 1 has launched nothing. Destroy a
- * handle only when its runs have finished and no graph that holds one will be replayed.
+ * does not change after that: runs of one handle may overlap on any streams and threads and be
+ * captured into CUDA graphs. A run is asynchronous on `stream` (cudaStream_t of the handle's
+ * device, NULL = legacy default), allocates no device memory and leaves the caller's current
+ * device as it was. Tensors are in memory of the handle's device. Strides count elements; 0 means
+ * packed. Inputs may be slices of one buffer. Return codes as above; a run that returns 1 has
+ * launched nothing. Destroy a handle only when its runs have finished and no graph that holds one
+ * will be replayed.
  * ---------------------------------------------------------------------------- */
 
 /* The norms before and after a block with its gate and residual scale, in one pass:
@@ -336,7 +337,8 @@ int ah_attn_create(int device, const ah_attn_desc* desc, int docs, const int64_t
                    int errlen);
 int ah_attn_run(ah_attn* h, const ah_attn_io* io, void* stream, char* err, int errlen);
 /* Reads and clears the device error word that the tensor-core kernel writes when a pipeline
- * wait runs out (0 = none; the run's output is then incomplete). Synchronises the device. */
+ * wait runs out (0 = none; the run's output is then incomplete). Synchronises the device, and the
+ * word is clear when it returns. */
 int ah_attn_status(ah_attn* h, uint32_t* status);
 void ah_attn_destroy(ah_attn* h);
 

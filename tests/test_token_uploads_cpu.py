@@ -120,3 +120,13 @@ def test_uploads_have_arrived_when_a_handle_is_there(fake):
     assert fake.fake_late() == 0
 
 
+def test_status_is_cleared_when_its_read_returns(fake):
+    """A later run's error word must not be wiped by a fill that is still on its way."""
+    attn = TokenAttention([0, 9], [0, 9], 1, 1, 64)
+    attn.run(*(BASE + i * MB for i in range(4)))
+    fake.fake_timeout()
+    assert attn.status() == 1
+    assert fake.fake_pending() == 0
+    fake.fake_timeout()
+    assert attn.status() == 1
+    assert attn.status() == 0
