@@ -32,6 +32,10 @@ void WriteShape(const std::vector<int64_t>& s, int64_t* out, int* rank) {
   for (size_t i = 0; i < s.size() && i < static_cast<size_t>(kMaxRank); ++i) out[i] = s[i];
 }
 
+// Copies from pageable memory and fills may return before they are on the device, ordered with the
+// legacy stream only, while a handle's first run may come at once on a non-blocking stream.
+cudaError_t UploadsArrived() { return cudaStreamSynchronize(cudaStreamLegacy); }
+
 size_t Elem(bool fp32) { return fp32 ? 4u : 2u; }
 
 bool LoadAndBuild(const char* path, int device, ah::Engine* eng, std::string* err) {
@@ -447,6 +451,7 @@ int ah_conv3x3_create(int device, int C, int M, const uint16_t* w, const float* 
   ce = c->tc ? ah::conv_tc_upload(w, bias, C, M, &c->tcw) : ah::simt_conv_upload(w, bias, C, M, &c->sw);
   if (ce == cudaSuccess) ce = cudaMalloc(&c->status, sizeof(uint32_t));
   if (ce == cudaSuccess) ce = cudaMemset(c->status, 0, sizeof(uint32_t));
+  if (ce == cudaSuccess) ce = UploadsArrived();
   if (ce != cudaSuccess) {
     CopyOut(std::string("conv weight upload failed: ") + cudaGetErrorString(ce), err, errlen);
     (void)cudaGetLastError();
@@ -492,6 +497,7 @@ int ah_conv3x3_create_algo(int device, int C, int M, const uint16_t* w, const fl
   ce = c->wino ? ah::wino_upload(w, bias, C, M, &c->ww) : ah::pair_upload(w, bias, C, M, &c->pw);
   if (ce == cudaSuccess) ce = cudaMalloc(&c->status, sizeof(uint32_t));
   if (ce == cudaSuccess) ce = cudaMemset(c->status, 0, sizeof(uint32_t));
+  if (ce == cudaSuccess) ce = UploadsArrived();
   if (ce != cudaSuccess) {
     CopyOut(std::string("conv weight upload failed: ") + cudaGetErrorString(ce), err, errlen);
     (void)cudaGetLastError();

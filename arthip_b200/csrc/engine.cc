@@ -186,6 +186,7 @@ bool Engine::Build(const onnx::Model& model, std::string& error) {
   if (!status_) {
     cudaError_t e = cudaMalloc(&status_, sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaMemset(status_, 0, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);  // the engine's stream does not wait for it
     if (e != cudaSuccess) {
       error = std::string("cudaMalloc of the status word failed: ") + cudaGetErrorString(e);
       return false;
@@ -775,6 +776,12 @@ bool Engine::UploadWeights(std::string& error) {
       error = std::string("cudaMalloc/cudaMemcpy of conv weights failed: ") + cudaGetErrorString(e);
       return false;
     }
+  }
+  // The engine's stream does not wait for the legacy stream, on which copies from pageable memory
+  // may still be on their way.
+  if (cudaError_t e = cudaStreamSynchronize(cudaStreamLegacy); e != cudaSuccess) {
+    error = std::string("upload of conv weights failed: ") + cudaGetErrorString(e);
+    return false;
   }
   weights_uploaded_ = true;
   return true;
