@@ -587,8 +587,10 @@ int ah_conv3x3_status(ah_conv* c, uint32_t* status) {
   cudaSetDevice(c->device);
   if (cudaDeviceSynchronize() != cudaSuccess) return 2;
   if (cudaMemcpy(status, c->status, sizeof(uint32_t), cudaMemcpyDeviceToHost) != cudaSuccess) return 2;
-  cudaMemset(c->status, 0, sizeof(uint32_t));
-  return 0;
+  if (*status == 0) return 0;
+  // The fill is waited for, so that it cannot wipe out what a later run reports.
+  if (cudaMemset(c->status, 0, sizeof(uint32_t)) != cudaSuccess) return 2;
+  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
 }
 
 void ah_conv3x3_destroy(ah_conv* c) {

@@ -1211,6 +1211,7 @@ bool Engine::CheckStatus(std::string& error) {
   }
   if (st != 0) {
     cudaMemset(status_, 0, sizeof(uint32_t));
+    cudaStreamSynchronize(cudaStreamLegacy);  // so that it cannot wipe out what a later frame reports
     error = "tensor-core conv kernel reported a timed-out pipeline wait (status " + std::to_string(st) + ")";
     return false;
   }

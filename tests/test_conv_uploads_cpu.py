@@ -113,3 +113,7 @@ def test_uploads_have_arrived_when_a_handle_is_there(lines):
     """Tensor-core, plain, Winograd and two-SM form: the first run may follow at once on a stream
     that nothing orders behind the uploads."""
     assert [l for l in lines if l.startswith("created")] == ["created 0"] * 4
+
+
+def test_status_is_cleared_when_its_read_returns(lines):
+    assert [l for l in lines if l.startswith("cleared")] == ["cleared 0"]
