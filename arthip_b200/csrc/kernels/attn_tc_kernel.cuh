@@ -515,14 +515,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           ptx::tmem_ld_32x32b_x16(from + c, o);
           ptx::tmem_wait_ld();
         }
-        if (r >= ntok[g]) continue;
-        uint4 q[2];
-        uint32_t* p = reinterpret_cast<uint32_t*>(q);
+        if (r < ntok[g]) {
+          uint4 q[2];
+          uint32_t* p = reinterpret_cast<uint32_t*>(q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          p[i] = n > 0 ? pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
-        *reinterpret_cast<uint4*>(dst + c) = q[0];
-        if (c + 8 < a.head_dim) *reinterpret_cast<uint4*>(dst + c + 8) = q[1];
+          for (int i = 0; i < 8; ++i)
+            p[i] = n > 0 ? pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
+          *reinterpret_cast<uint4*>(dst + c) = q[0];
+          if (c + 8 < a.head_dim) *reinterpret_cast<uint4*>(dst + c + 8) = q[1];
+        }
+        __syncwarp();  // the next load wants the whole warp together, lanes behind the last query too
       }
     }
   }
