@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         for (int c = 0; c < a.head_dim; c += 16) {
           uint32_t o[8];
           ptx::tmem_ld_16x256b_x2(to + c, o);
-          ptx::tmem_wait_ld();
+          ptx::tmem_wait_ld(o);
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink[e >> 1 & 1]);
           ptx::tmem_st_16x256b_x2(to + c, o);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         uint32_t o[32];
         if (n > 0) {
           ptx::tmem_ld_32x32b_x16(from + c, o);
-          ptx::tmem_wait_ld();
+          ptx::tmem_wait_ld_x16(o);
         }
         if (r < ntok[g]) {
           uint4 q[2];
