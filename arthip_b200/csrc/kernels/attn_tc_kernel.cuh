@@ -488,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       ptx::tmem_wait_st();
       arrive(p_ready + g);
     }
+    ptx::tmem_wait_st();  // a step that a wait ended early may have left stores under way
     if (n > 0) {
       if constexpr (L::kOwnP)
         await(o_done + g, (n - 1) & 1);
