@@ -13,6 +13,7 @@
 #include "ep_partition.h"
 #include "fp16_host.h"
 #include "kernels/kernels.h"
+#include "kernels/tokens.h"
 
 namespace {
 
@@ -606,6 +607,10 @@ void ah_conv3x3_destroy(ah_conv* c) {
 
 void ah_test_set_conv_fault_hook(int wait_limit_ms, int stall_row) {
   ah::conv_tc_set_test_hook(wait_limit_ms, stall_row);
+}
+
+void ah_test_set_attn_fault_hook(int wait_limit_ms, int stall_load) {
+  ah::attn_tc_set_test_hook(wait_limit_ms, stall_load);
 }
 
 // ---------------------------------------------------------------------------

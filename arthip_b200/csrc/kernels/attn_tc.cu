@@ -3,11 +3,17 @@
 // parameter, so a captured launch keeps its own.
 #include "attn_tc_kernel.cuh"
 
+#include <atomic>
+
 #include <cuda.h>
 
 namespace ah {
 
 namespace {
+
+// Failure-path test hook (ah_test_set_attn_fault_hook): 0 = off.
+std::atomic<int> g_test_wait_ms{0};
+std::atomic<int> g_test_stall_load{-1};
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -42,6 +48,12 @@ bool encode(EncodeTiledFn fn, CUtensorMap* map, int dtype, const void* p, int di
 
 }  // namespace
 
+void attn_tc_set_test_hook(int wait_limit_ms, int stall_load) {
+  const bool on = wait_limit_ms > 0 && wait_limit_ms <= 4000 && stall_load >= 0;
+  g_test_stall_load.store(on ? stall_load : -1, std::memory_order_relaxed);
+  g_test_wait_ms.store(on ? wait_limit_ms : 0, std::memory_order_relaxed);
+}
+
 cudaError_t attn_tc_launch(const AttnArgs& a, int dtype, cudaStream_t s, std::string* err) {
   const EncodeTiledFn fn = encode_fn();
   if (!fn) {
@@ -50,6 +62,9 @@ cudaError_t attn_tc_launch(const AttnArgs& a, int dtype, cudaStream_t s, std::st
   }
   AttnTcArgs args;
   args.a = a;
+  const int hook_ms = g_test_wait_ms.load(std::memory_order_relaxed);
+  args.wait_limit_ns = hook_ms > 0 ? static_cast<unsigned long long>(hook_ms) * 1000000ull : ptx::kWaitLimitNs;
+  args.stall_load = hook_ms > 0 ? g_test_stall_load.load(std::memory_order_relaxed) : -1;
   if (!encode(fn, &args.q, dtype, a.q, a.head_dim, a.q_total, a.q_tok, a.q_heads, a.q_head, err) ||
       !encode(fn, &args.k, dtype, a.k, a.head_dim, a.k_total, a.k_tok, a.kv_heads, a.k_head, err) ||
       !encode(fn, &args.v, dtype, a.v, a.head_dim, a.k_total, a.v_tok, a.kv_heads, a.v_head, err))

@@ -48,6 +48,8 @@ namespace ah {
 struct AttnTcArgs {
   CUtensorMap q, k, v;  // {head_dim, tokens, heads}, box {64, 128, 1}, 128B swizzle
   AttnArgs a;
+  unsigned long long wait_limit_ns;  // bound of every pipeline wait (4 s)
+  int stall_load;  // failure-path test: the load (K and V of each tile in turn) that never comes, or -1
 };
 
 namespace attn_tc {
@@ -200,18 +202,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       for (; issued < 2 * ntiles; ++issued) {  // K and V of each tile in turn
         const int slot = issued % L::kSlots, use = issued / L::kSlots;
-        if (!ptx::mbar_wait_short(ptx::smem_u32(empty + slot), (use & 1) ^ 1, abort_flag)) break;
+        if (!ptx::mbar_wait_short(ptx::smem_u32(empty + slot), (use & 1) ^ 1, abort_flag, args.wait_limit_ns)) break;
         const uint32_t fb = ptx::smem_u32(full + slot);
         ptx::mbar_arrive_expect_tx(fb, L::kTile);
+        if (issued == args.stall_load) continue;
         const CUtensorMap* map = issued & 1 ? &args.v : &args.k;
         for (int c = 0; c < NCH; ++c)
           ptx::tma_load_3d(ptx::smem_u32(smem + L::kRing + slot * L::kTile + c * kChunkBytes), map, fb, c * 64,
                            doc.k0 + (issued >> 1) * kTcKeys, kvh);
       }
       // Nothing may be in flight when the CTA ends, which after a wait that ran out it might.
-      if (ntiles > 0) ptx::mbar_wait_short(ptx::smem_u32(q_full), 0, &never_abort);
+      if (ntiles > 0) ptx::mbar_wait_short(ptx::smem_u32(q_full), 0, &never_abort, args.wait_limit_ns);
       for (int i = max(0, issued - L::kSlots); i < issued; ++i)
-        ptx::mbar_wait_short(ptx::smem_u32(full + i % L::kSlots), (i / L::kSlots) & 1, &never_abort);
+        ptx::mbar_wait_short(ptx::smem_u32(full + i % L::kSlots), (i / L::kSlots) & 1, &never_abort, args.wait_limit_ns);
     }
     __syncwarp();
   } else if (warp >= kProductWarp) {
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int n = tiles[g];
     auto slot_words = [&](int seq) { return static_cast<uint32_t>(seq % L::kSlots * (L::kTile >> 4)); };
     auto await = [&](uint64_t* bar, int parity) {
-      return ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag);
+      return ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag, args.wait_limit_ns);
     };
     auto wait_full = [&](int seq) { return await(full + seq % L::kSlots, (seq / L::kSlots) & 1); };
     auto release = [&](int seq) { ptx::mma_commit(ptx::smem_u32(empty + seq % L::kSlots)); };
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       // No product may be running when tensor memory is freed.
       ptx::mma_commit(ptx::smem_u32(drained + g));
-      ptx::mbar_wait_short(ptx::smem_u32(drained + g), 0, &never_abort);
+      ptx::mbar_wait_short(ptx::smem_u32(drained + g), 0, &never_abort, args.wait_limit_ns);
     }
     __syncwarp();
   } else {
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     bool ok = true;
     auto await = [&](uint64_t* bar, int parity) {  // the same answer in all lanes
-      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag));
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait_short(ptx::smem_u32(bar), parity, abort_flag, args.wait_limit_ns));
     };
     auto arrive = [&](uint64_t* bar) {
       ptx::tc_fence_before();

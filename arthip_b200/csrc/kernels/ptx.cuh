@@ -102,11 +102,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // The same for short waits on a kernel's critical path: some tries before the clock is read.
-__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                unsigned long long limit_ns) {
 #pragma unroll 1
   for (int i = 0; i < 32; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, abort_flag);
+  return mbar_wait(bar, parity, abort_flag, limit_ns);
 }
 
 // ---------------------------------------------------------------------------

@@ -125,5 +125,7 @@ constexpr int kTcKeys = 128;
 inline bool attn_tc_head_pairs(int group) { return group % 2 == 0; }
 inline int attn_tc_item_tokens(int group) { return attn_tc_head_pairs(group) ? kTcRows : 2 * kTcRows; }
 cudaError_t attn_tc_launch(const AttnArgs& a, int dtype, cudaStream_t s, std::string* err);
+// Bounds every wait of later launches by wait_limit_ms and leaves out load `stall_load` of each CTA.
+void attn_tc_set_test_hook(int wait_limit_ms, int stall_load);
 
 }  // namespace ah

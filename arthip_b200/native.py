@@ -75,6 +75,7 @@ SIGNATURES: dict[str, tuple] = {
     "ah_attn_status": (_i32, [_vp, _u32p]),
     "ah_attn_destroy": (None, [_vp]),
     "ah_test_set_conv_fault_hook": (None, [_i32, _i32]),
+    "ah_test_set_attn_fault_hook": (None, [_i32, _i32]),
     "ah_convert_float_to_float16": (_i32, [_vp, _sz, _i32, _cp, _i32, _i32, _vp, _sz, _szp, _cp, _i32]),
     "ah_load_onnx": (_i32, [_vp, _sz, _cp, _i64, _i64, _vp, _sz, _szp, _cp, _i32]),
     "ah_vs_model_create": (_i32, [_vp, _vp, _sz, _cp, _vp, ctypes.POINTER(_vp), _cp, _i32]),

@@ -348,6 +348,9 @@ void ah_attn_destroy(ah_attn* h);
  * loading it, so the kernel must report a timed-out wait through its status word without
  * faulting. Any other arguments (e.g. 0, -1) turn it off, which is the default. */
 void ah_test_set_conv_fault_hook(int wait_limit_ms, int stall_row);
+/* The same for launches of the tcgen05 attention kernel: every CTA arms the slot of its load
+ * `stall_load` (keys and values of each tile in turn: 0, 1, 2, ...) without loading it. */
+void ah_test_set_attn_fault_hook(int wait_limit_ms, int stall_load);
 
 /* ------------------------------------------------------------------------------
  * VapourSynth filter hip.Model and its loading path (src/vapoursynth/vs_hip.cpp,
