@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 
@@ -69,3 +71,56 @@ def test_attention_wait_that_runs_out_is_reported_and_recovers(stall, d, bias):
     assert op.status() == 0
     ref, bound = attn_ref(q, k, v, [0, 300], [0, 700], d ** -0.5, slopes=slopes, q_pos=q_pos, k_pos=k_pos)
     check(out, ref, bound, "fp16", "after recovery")
+
+
+def infinite_key(nq, nk, d, dtype, seed):
+    """q, k, v of one head, key 77 with an infinity in element 5 where every query is 1 to 2 or -1
+    to -2, and which queries see it as +inf."""
+    g = gen(seed)
+    q, k, v = (randn(g, (n, 1, d), dtype) for n in (nq, nk, nk))
+    sign = torch.where(torch.rand(nq, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    sign[0], sign[-1] = 1.0, -1.0
+    q[:, 0, 5] = (sign * (1 + torch.rand(nq, generator=g, device="cuda"))).to(q.dtype)
+    k[77, 0, 5] = math.inf
+    return q, k, v, sign > 0
+
+
+# Queries, keys: the tcgen05 form, 64 rows a block with and without a cluster, 16 rows likewise
+INFINITE = [(200, 300, "tc"), (200, 300, "mma"), (64, 4000, "mma"), (3, 300, "mma"), (3, 9000, "mma")]
+
+
+@pytest.mark.parametrize("nq,nk,algo", INFINITE)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attention_infinite_key(nq, nk, algo, d, dtype):
+    """A score of +inf makes its row NaN, as inf - inf in its softmax does; one of -inf is a key of no
+    weight."""
+    q, k, v, plus = infinite_key(nq, nk, d, dtype, nq + nk)
+    out = torch.zeros_like(q)
+    op = TokenAttention([0, nq], [0, nk], 1, 1, d, dtype=dtype, algo=algo)
+    op.run(ptr(q), ptr(k), ptr(v), ptr(out), stream=stream())
+    assert torch.isnan(out[plus]).all()
+    rest = [torch.cat([t[:77], t[78:]]) for t in (k, v)]
+    ref, bound = attn_ref(q[~plus], *rest, [0, int((~plus).sum())], [0, nk - 1], d ** -0.5, dtype=dtype)
+    check(out[~plus], ref, bound, dtype, "rows of a score of -inf")
+
+
+@pytest.mark.parametrize("nq,nk,algo", INFINITE)
+@pytest.mark.parametrize("cap", [5.0, 1000.0])
+def test_attention_infinite_key_under_a_cap(nq, nk, algo, cap):
+    """A cap makes an infinite score the cap, or minus the cap."""
+    q, k, v, plus = infinite_key(nq, nk, 64, "fp16", nq + nk)
+    out = torch.zeros_like(q)
+    op = TokenAttention([0, nq], [0, nk], 1, 1, 64, cap=cap, algo=algo)
+    op.run(ptr(q), ptr(k), ptr(v), ptr(out), stream=stream())
+    if cap == 1000.0:  # exp(-990) of anything else is left: the row is that key's value, or without it
+        assert torch.equal(out[plus], v[77:78].expand(int(plus.sum()), 1, 64))
+        rest = [torch.cat([t[:77], t[78:]]) for t in (k, v)]
+        ref, bound = attn_ref(q[~plus], *rest, [0, int((~plus).sum())], [0, nk - 1], 0.125, cap)
+        check(out[~plus], ref, bound, "fp16", "rows of a score of -cap")
+    else:
+        # 2^9 gives scores of some 64 or more, 12 caps: 1 - tanh 12 = 8e-11. (The infinite score is the
+        # cap exactly; the bound's term for a product sum, 68 E 2^9 2 / 8 = 5e-4, is to spare.)
+        k[77, 0, 5] = 2.0 ** 9
+        ref, bound = attn_ref(q, k, v, [0, nq], [0, nk], 0.125, cap)
+        check(out, ref, bound, "fp16", "rows of a score of the cap")
