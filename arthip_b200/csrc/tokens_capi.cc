@@ -302,8 +302,11 @@ int ah_norm_run(ah_norm* h, const ah_norm_io* io, void* stream, char* err, int e
   if (!h || !io) return Fail("invalid norm run arguments", err, errlen);
   if (io->rows < 0 || io->rows_per_gate < 1 || io->rows_per_mod < 1)
     return Fail("norm: rows must not be negative, rows_per_gate and rows_per_mod at least 1", err, errlen);
-  if (!io->x || (!io->out && !io->norm)) return Fail("norm: x and one of out and norm are needed", err, errlen);
-  if ((io->gate || io->out) && !io->y) return Fail("norm: out and gate need the block output y", err, errlen);
+  // Tensors of no rows may be null.
+  if (io->rows > 0 && (!io->x || (!io->out && !io->norm)))
+    return Fail("norm: x and one of out and norm are needed", err, errlen);
+  if (io->rows > 0 && (io->gate || io->out) && !io->y)
+    return Fail("norm: out and gate need the block output y", err, errlen);
   const int64_t C = h->args.C, rows = io->rows;
   auto pitch = [&](int64_t s) { return s ? s : C; };
   const int64_t grows = rows ? (rows - 1) / io->rows_per_gate + 1 : 0;
@@ -408,7 +411,8 @@ int ah_rope_create(int device, const ah_rope_desc* d, ah_rope** out, char* err, 
 
 int ah_rope_run(ah_rope* h, int64_t tokens, const float* positions, const ah_rope_io* q, const ah_rope_io* k,
                 void* stream, char* err, int errlen) try {
-  if (!h || !positions || (!q && !k)) return Fail("invalid rope run arguments", err, errlen);
+  if (!h || (tokens > 0 && (!positions || (!q && !k))))  // tensors of no tokens may be null
+    return Fail("invalid rope run arguments", err, errlen);
   if (tokens < 0 || tokens > (int64_t(1) << 31) - 1) return Fail("rope: tokens must be 0..2^31-1", err, errlen);
   if (!Aligned(positions, 4)) return Fail("rope: positions must be 4-byte aligned", err, errlen);
   const int D = h->table.head_dim;
@@ -420,7 +424,7 @@ int ah_rope_run(ah_rope* h, int64_t tokens, const float* positions, const ah_rop
     const ah_rope_io* io = w ? k : q;
     if (!io) continue;
     if (io->heads < 1 || io->heads > 1024) return Fail("rope: heads must be 1..1024", err, errlen);
-    if (!io->in || !io->out) return Fail("rope: null tensor", err, errlen);
+    if (tokens > 0 && (!io->in || !io->out)) return Fail("rope: null tensor", err, errlen);
     const int64_t packed = static_cast<int64_t>(io->heads) * D;
     in[w] = View{io->in, tokens, io->in_token_stride ? io->in_token_stride : packed, io->heads,
                  io->in_head_stride ? io->in_head_stride : D, D};

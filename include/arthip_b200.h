@@ -213,10 +213,10 @@ int ah_conv3x3_run_noalloc(int device, int C, int M, const uint16_t* w_oihw_f16,
  * does not change after that: runs of one handle may overlap on any streams and threads and be
  * captured into CUDA graphs. A run is asynchronous on `stream` (cudaStream_t of the handle's
  * device, NULL = legacy default), allocates no device memory and leaves the caller's current
- * device as it was. Tensors are in memory of the handle's device. Strides count elements; 0 means
- * packed. Inputs may be slices of one buffer. Return codes as above; a run that returns 1 has
- * launched nothing. Destroy a handle only when its runs have finished and no graph that holds one
- * will be replayed.
+ * device as it was. Tensors are in memory of the handle's device; those of no tokens may be NULL.
+ * Strides count elements; 0 means packed. Inputs may be slices of one buffer. Return codes as
+ * above; a run that returns 1 has launched nothing. Destroy a handle only when its runs have
+ * finished and no graph that holds one will be replayed.
  * ---------------------------------------------------------------------------- */
 
 /* The norms before and after a block with its gate and residual scale, in one pass:

@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from arthip_b200.native import lib  # noqa: E402
-from arthip_b200.token_ops import TokenAttention  # noqa: E402
+from arthip_b200.token_ops import AxisRotary, TokenAttention, TokenNorm  # noqa: E402
 from test_token_ops_gpu import gen, ptr, randn, run_attn, run_norm, stream  # noqa: E402
 from token_ref import attn_ref, check  # noqa: E402
 
@@ -124,3 +124,13 @@ def test_attention_infinite_key_under_a_cap(nq, nk, algo, cap):
         k[77, 0, 5] = 2.0 ** 9
         ref, bound = attn_ref(q, k, v, [0, nq], [0, nk], 0.125, cap)
         check(out, ref, bound, "fp16", "rows of a score of the cap")
+
+
+def test_runs_of_no_tokens_do_nothing():
+    x = torch.empty(0, 64, dtype=torch.float16, device="cuda")
+    pos = torch.empty(1, 0, device="cuda")
+    assert x.data_ptr() == 0
+    TokenNorm(64).run(0, ptr(x), ptr(x), ptr(x), ptr(x), stream=stream())
+    AxisRotary(64, [64]).run(0, ptr(pos), ptr(x), 1, stream=stream())
+    TokenAttention([0, 0], [0, 0], 1, 1, 64).run(ptr(x), ptr(x), ptr(x), ptr(x), stream=stream())
+    torch.cuda.synchronize()
