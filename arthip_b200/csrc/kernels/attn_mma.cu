@@ -21,15 +21,12 @@
 // partial results are joined through distributed shared memory, so that no workspace is needed
 // and the order of the sums is fixed; and 64 rows with all their keys in one CTA, which takes
 // some key heads one after another, the next one's loads under way, and writes its rows itself.
-#include "ptx.cuh"
 #include "token_common.cuh"
 #include "tokens.h"
 
 #include <algorithm>
 
 #include <cooperative_groups.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace ah {
 
@@ -40,19 +37,6 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kStages = 3;
 constexpr float kWeightShift = 6.f;  // weights are 2^(x - max + 6): a wider range above fp16's smallest
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -85,17 +69,6 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 // 16 bytes into shared memory, or zeros.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 enum Form : int { kFew = 0, kWideShared = 1, kWideAlone = 2 };
@@ -221,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
 #pragma unroll
   for (int p = 0; p < kStages - 1; ++p) {
     if (p < steps) load_step(p);
-    cp_async_commit();
+    copies_commit();
   }
 
   // This thread's two rows.
@@ -275,10 +248,10 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
   uint32_t qf[kKD][4];
   int tile = tile0;
   for (int step = 0; step < steps; ++step) {
-    cp_async_wait<kStages - 2>();
+    copies_wait<kStages - 2>();
     __syncthreads();
     if (step + kStages - 1 < steps) load_step(step + kStages - 1);
-    cp_async_commit();
+    copies_commit();
     uint8_t* st = sStage + step % kStages * L::kStage;
     if (tile == tile0) {
       const uint32_t sq =
@@ -418,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, FORM == kWideAlone && DP == 32 ? 4 :
       }
     }
   }
-  cp_async_wait<0>();
+  copies_wait<0>();
   if constexpr (FORM == kWideAlone) return;
   const int kvh = kvh0;
   join_lanes();

@@ -37,11 +37,7 @@
 #pragma once
 
 #include "token_common.cuh"
-#include "ptx.cuh"
 #include "tokens.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace ah {
 
@@ -76,25 +72,6 @@ struct Smem {
   static constexpr int kColO = 256, kColP = kOwnP ? 384 : 0, kStrideP = kOwnP ? 64 : 128;
   static constexpr int kBytes = kBars + 256 + 1024;    // and room to align to 1024
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <typename T>
 constexpr bool kIsBf16 = false;

@@ -1,5 +1,6 @@
-// What the token kernels share: the capped score of attention, asynchronous copies of vectors and
-// of rows of any alignment, and launch attributes.
+// What the token kernels share: conversions of the two element types, the exponential and the capped
+// score of attention, asynchronous copies of vectors and of rows of any alignment, and launch
+// attributes.
 #pragma once
 
 #include "ptx.cuh"
@@ -7,9 +8,46 @@
 
 #include <atomic>
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 namespace ah {
+
+// fp16 and bf16, one at a time and in pairs.
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ void from_f(float v, __half* o) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f2(float a, float b, __half2* o) { *o = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void from_f2(float a, float b, __nv_bfloat162* o) { *o = __floats2bfloat162_rn(a, b); }
+
+template <typename T>
+struct Two;
+template <>
+struct Two<__half> {
+  using type = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+// Two values rounded to T, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typename Two<T>::type v;
+  from_f2(lo, hi, &v);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // How scores are capped, cap * tanh(s / cap), in powers of two:
 //   kCapExp     cap (1 - 2 / (1 + exp(2 s / cap))), good to a few units of 2^-24 cap
@@ -32,10 +70,8 @@ __device__ __forceinline__ float rcp_fast(float x) {
 template <int FORM>
 __device__ __forceinline__ uint64_t attn_capped2(uint64_t s, const AttnArgs& a) {
   auto both = [](float v) { return ptx::pack_f2(v, v); };
-  float2 e = ptx::unpack_f2(ptx::mul_f2(s, both(a.cap_exp)));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
-  const float2 d = ptx::unpack_f2(ptx::add_f2(ptx::pack_f2(e.x, e.y), both(1.f)));
+  const float2 e = ptx::unpack_f2(ptx::mul_f2(s, both(a.cap_exp)));
+  const float2 d = ptx::unpack_f2(ptx::add_f2(ptx::pack_f2(exp2_fast(e.x), exp2_fast(e.y)), both(1.f)));
   const uint64_t x =
       ptx::fma_f2(ptx::pack_f2(rcp_fast(d.x), rcp_fast(d.y)), both(-2.f * a.cap_log2), both(a.cap_log2));
   if constexpr (FORM == kCapSeries) {

@@ -24,34 +24,13 @@
 #include <algorithm>
 #include <atomic>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 namespace ah {
 namespace token_norm {
 
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-__device__ __forceinline__ void from_f(float v, __half* o) { *o = __float2half_rn(v); }
-__device__ __forceinline__ void from_f(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f2(float a, float b, __half2* o) { *o = __floats2half2_rn(a, b); }
-__device__ __forceinline__ void from_f2(float a, float b, __nv_bfloat162* o) { *o = __floats2bfloat162_rn(a, b); }
-
-template <typename T>
-struct Two;
-template <>
-struct Two<__half> {
-  using type = __half2;
-};
-template <>
-struct Two<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
-
+// Vectors of 4 or 8 elements.
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
+  static_assert(V % 4 == 0, "weights are read four at a time");
   T e[V];
 };
 
@@ -62,32 +41,24 @@ __device__ __forceinline__ Vec<T, V> load(const T* p) {
 
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Vec<T, V>& u, float (&f)[V]) {
-  if constexpr (V % 2 == 0) {
-    const auto* p = reinterpret_cast<const typename Two<T>::type*>(&u);
+  const auto* p = reinterpret_cast<const typename Two<T>::type*>(&u);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float2 t = to_f2(p[i]);
-      f[2 * i] = t.x, f[2 * i + 1] = t.y;
-    }
-  } else {
-    f[0] = to_f(u.e[0]);
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 t = to_f2(p[i]);
+    f[2 * i] = t.x, f[2 * i + 1] = t.y;
   }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
   Vec<T, V> u;
-  if constexpr (V % 2 == 0) {
-    auto* q = reinterpret_cast<typename Two<T>::type*>(&u);
+  auto* q = reinterpret_cast<typename Two<T>::type*>(&u);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) from_f2(f[2 * i], f[2 * i + 1], q + i);
-  } else {
-    from_f(f[0], &u.e[0]);
-  }
+  for (int i = 0; i < V / 2; ++i) from_f2(f[2 * i], f[2 * i + 1], q + i);
   *reinterpret_cast<Vec<T, V>*>(p) = u;
 }
 
-// V floats of a weight array, 16 bytes at a time where V allows, or `fill` without one.
+// V floats of a weight array, 16 bytes at a time, or `fill` without one.
 template <int V>
 __device__ __forceinline__ void load_weight(const float* p, int c, float fill, float (&f)[V]) {
   if (!p) {
@@ -96,15 +67,10 @@ __device__ __forceinline__ void load_weight(const float* p, int c, float fill, f
     return;
   }
   p += c;
-  if constexpr (V % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
-      f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = __ldg(p + i);
+  for (int i = 0; i < V; i += 4) {
+    const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+    f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
   }
 }
 

@@ -16,35 +16,12 @@
 
 #include <algorithm>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 namespace ah {
 
 namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTableBytes = 16384;  // cosines and sines of a block's tokens
-
-__device__ __forceinline__ float2 unpack(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ float2 unpack(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-__device__ __forceinline__ void pack(float2 f, __half2* o) { *o = __float22half2_rn(f); }
-__device__ __forceinline__ void pack(float2 f, __nv_bfloat162* o) { *o = __float22bfloat162_rn(f); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_f(float v, __half* o) { *o = __float2half_rn(v); }
-__device__ __forceinline__ void from_f(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
-
-template <typename T>
-struct Two;
-template <>
-struct Two<__half> {
-  using type = __half2;
-};
-template <>
-struct Two<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
 
 // How a head is cut into the units that one thread turns:
 //   kUnitPairs   8 elements, four adjacent pairs
@@ -142,13 +119,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeTable t, c
       T2* pa = reinterpret_cast<T2*>(v);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack(pa[j]);
+        const float2 x = to_f2(pa[j]);
         if constexpr (UNIT == kUnitPairs) {
-          pack(make_float2(x.x * c[j].x - x.y * c[j].y, x.x * c[j].y + x.y * c[j].x), pa + j);
+          from_f2(x.x * c[j].x - x.y * c[j].y, x.x * c[j].y + x.y * c[j].x, pa + j);
         } else {
-          const float2 c0 = c[2 * j], c1 = c[2 * j + 1], y = unpack(pa[4 + j]);
-          pack(make_float2(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y), pa + j);
-          pack(make_float2(x.x * c0.y + y.x * c0.x, x.y * c1.y + y.y * c1.x), pa + 4 + j);
+          const float2 c0 = c[2 * j], c1 = c[2 * j + 1], y = to_f2(pa[4 + j]);
+          from_f2(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y, pa + j);
+          from_f2(x.x * c0.y + y.x * c0.x, x.y * c1.y + y.y * c1.x, pa + 4 + j);
         }
       }
       if constexpr (UNIT == kUnitHalves) *reinterpret_cast<uint4*>(out + e1) = v[1];
