@@ -134,3 +134,16 @@ def test_runs_of_no_tokens_do_nothing():
     AxisRotary(64, [64]).run(0, ptr(pos), ptr(x), 1, stream=stream())
     TokenAttention([0, 0], [0, 0], 1, 1, 64).run(ptr(x), ptr(x), ptr(x), ptr(x), stream=stream())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("nq", [3, 70])
+def test_attention_widest_clusters(nq, d):
+    """Few blocks on long caches: the keys are shared out over clusters of sixteen."""
+    run_attn([nq], [20000], 1, 1, d, "bf16", causal=True, lens=[19001], seed=d)
+
+
+@pytest.mark.parametrize("hq,hk", [(1024, 1), (1024, 1024), (1023, 341)])
+@pytest.mark.parametrize("nq", [1, 130])
+def test_attention_most_heads(hq, hk, nq):
+    run_attn([nq], [140], hq, hk, 8, causal=True, seed=hq + nq)
