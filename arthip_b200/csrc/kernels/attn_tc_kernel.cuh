@@ -11,8 +11,10 @@
 // wait for S, load it or look for its maximum. Four threads share a row (the 16-lane loads of
 // tensor memory give each of them every fourth pair of columns) and find its maximum with two
 // shuffles. Half of the scores are loaded a second time rather than kept, which holds a thread
-// to the 96 registers that 19 warps leave it. Warp 16 issues the TMA loads of key and value
-// tiles into a ring, warps 17 and 18 the products of one tile each.
+// to the 96 registers that 19 warps leave it; with a cap or a bias it is not quite enough, and 32
+// to 132 bytes a thread are spilled (1.4% of the instructions of a capped and biased run). Warp 16
+// issues the TMA loads of key and value tiles into a ring, warps 17 and 18 the products of one tile
+// each.
 //
 // Heads of up to 64 have room for P beside S: S of the next keys is computed as soon as this
 // one has been loaded into registers, and a softmax warp never waits for the round trip
@@ -28,12 +30,13 @@
 //
 // Every wait is bounded; one that runs out ends the CTA and sets the status word.
 //
-// Bound: the special function unit, one exponential a score at 16 per clock, and close behind it
-// the issue of the 5.9 instructions that a score takes. 32400 tokens, 8 heads of 64: 2.78 ms, 76%
-// of the unit's rate (exponentials alone 1.92 ms, products 1.27 ms). Tried beside this: issue by
-// lane 0 instead of an elected thread 4.0 ms; two softmax warps per scheduler, whole rows, 3.1;
-// keys 64 at a time with two buffers of S 3.5; a quarter of the exponentials as polynomials on
-// the FMA pipe 2.93.
+// Bound: latency, with the special function unit (one exponential a score at 16 per clock) and the
+// issue of the 5.9 instructions that a score takes nearest to full. 32400 tokens, 8 heads of 64: 2.78
+// to 3.03 ms (exponentials alone 1.92 ms at 1.85 GHz, products 1.27 ms); counted at 2.94 ms, the unit
+// is 73% busy and issue 0.54. Capped and biased, 128 elements a head: unit 60%, issue 0.42. Tried
+// beside this: issue by lane 0 instead of an elected thread 4.0 ms; two softmax warps per scheduler,
+// whole rows, 3.1; keys 64 at a time with two buffers of S 3.5; a quarter of the exponentials as
+// polynomials on the FMA pipe 2.93.
 #pragma once
 
 #include "token_common.cuh"

@@ -163,7 +163,9 @@ cudaError_t launch(const RopeTable& t, const RopeArgs& a, int num_sms, cudaStrea
 // Heads of any cut, width, stride and alignment: a warp takes a run of a token's heads into shared
 // memory in 16-byte pieces, one run ahead, turns its pairs there and sends them out the same way.
 // A lane's pairs are every 32nd of a head, their cosines and sines in registers for all heads of
-// the token. (Turned in global memory, pair by pair, such heads ran at 31% of the copy rate.)
+// the token. Pairs are turned element by element there, so short heads, which leave lanes without a
+// pair, cost most: 48 heads of 128 run at 63% of the copy rate (turned in global memory at 31%), 16
+// of 64 in sections of 22, 20 and 22 at 47%, 16 of 30 at 23%.
 struct RopeRuns {
   int slot = 0;         // bytes of a run in shared memory
   int heads[2] = {};    // of a run of q, of k

@@ -174,6 +174,13 @@ int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // its time does not fall, while the mma.sync kernel cuts its keys up further, at about 1.7 times
 // the work and 8 us for the joining: 1024 queries on 8192 keys, 4 heads of 64, 111 us and 59;
 // 1024 on 1024, 12 heads of 64, 23 and 33.
+// What it does not know: a causal mask, which halves the keys of both kernels, and how far a cache
+// is filled. Over documents of 96 to 768 tokens (131072 in all, 4 heads) its choice costs at most
+// 27% with a causal mask (256 of 32: 108 us, the other kernel 85) and 19% without (192 of 64: 173
+// and 145), and nothing at 38 of 42 sizes; but 64 causal queries on each of 16 caches of 4096 keys
+// filled to a quarter, heads of 128, take 61 us where the tcgen05 kernel would take 21, and on each
+// of 128 caches of 512, heads of 64, 23 us where the mma.sync kernel would take 13. A caller that
+// knows names the kernel (algo).
 class KernelChoice {
  public:
   KernelChoice(const std::vector<ah::AttnDoc>& docs, int algo, int q_heads, int kv_heads, int head_dim, int num_sms)

@@ -201,9 +201,13 @@ class TokenAttention(_Handle):
     ``mask``: "full", or "causal" (aligned to the last key), with ``prefix[i]`` first keys that
     every query of document i sees. ``cap``: scores become ``cap * tanh(score / cap)``.
     ``slopes`` [q_heads][axes]: ``slope * |q position - k position|`` is taken off the scores
-    for each axis. ``scale`` defaults to ``head_dim ** -0.5``. ``algo``: "auto" takes for each
-    document the kernel that is expected to be done sooner; "mma" and "tc" the mma.sync and the
-    tcgen05 one for all."""
+    for each axis. The softmax weights are rounded to ``dtype`` before they multiply the values;
+    scores and sums are fp32. ``scale`` defaults to ``head_dim ** -0.5``. ``algo``: "auto" takes
+    for each document the kernel that is expected to be done sooner, reckoning with whole
+    documents and full caches; "mma" and "tc" the mma.sync and the tcgen05 one for all.
+
+    A handle is a plan for these lengths (made in 46 us for a few documents, 0.1 ms for 2000, 0.8 ms
+    for 32000); keys in use that change from run to run are ``k_lens_ptr`` of :meth:`run`."""
 
     _destroy = "ah_attn_destroy"
 

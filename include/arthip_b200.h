@@ -206,8 +206,9 @@ int ah_conv3x3_run_noalloc(int device, int C, int M, const uint16_t* w_oihw_f16,
  * Token operators on device tensors (no counterpart in the reference; additions of this
  * library), for the layers that stand between conv layers in attention-based restoration
  * models. A token is a pixel or patch of a frame; rows are tokens, so a conv layer's NHWC
- * frame is [tokens][channels] as it stands. Element types: 0 = fp16, 1 = bf16. Sums,
- * statistics and softmax weights' sums are fp32.
+ * frame is [tokens][channels] as it stands. Element types: 0 = fp16, 1 = bf16. Sums, statistics
+ * and scores are fp32, outputs are rounded once; attention's softmax weights are rounded to the
+ * element type before they multiply the values, their sum is not.
  *
  * A handle holds uploaded parameters only, has them on the device when its creation returns, and
  * does not change after that: runs of one handle may overlap on any streams and threads and be
@@ -299,7 +300,9 @@ void ah_rope_destroy(ah_rope* h);
  *   s -= sum over axes of slopes[head][axis] * |q_position - k_position|
  * mask 0: every key of the document. mask 1 (causal): keys j <= i + (keys - queries), counted
  * in the document, and the document's first prefix keys. A query that sees no key gets zeros.
- * Query head h reads key head h / (q_heads / kv_heads). */
+ * Query head h reads key head h / (q_heads / kv_heads). The weights exp(s - max) are rounded to the
+ * element type before they multiply v (half a step of each, which adds about as much to an output's
+ * error as its own rounding does); their sum is taken before that, in fp32. */
 typedef struct {
   int dtype;
   int q_heads, kv_heads;
@@ -308,8 +311,9 @@ typedef struct {
   float cap;    /* 0 = none */
   int mask;
   int axes;     /* of the distance bias, 0..3 */
-  int algo;     /* 0: for each document the kernel that is expected to be done sooner;
-                 * 1: mma.sync for all; 2: tcgen05 for all that have queries and keys */
+  int algo;     /* 0: for each document the kernel that is expected to be done sooner, reckoned with
+                 * all its queries and keys (no causal mask, no k_lens); 1: mma.sync for
+                 * all; 2: tcgen05 for all that have queries and keys */
 } ah_attn_desc;
 /* q, out [q_offsets[docs]][q_heads][head_dim]; k, v [k_offsets[docs]][kv_heads][head_dim], by
  * strides that are multiples of 8 elements, from 16-byte aligned pointers; out overlaps no
