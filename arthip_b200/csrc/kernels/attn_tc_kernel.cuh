@@ -31,7 +31,7 @@
 // Every wait is bounded; one that runs out ends the CTA and sets the status word.
 //
 // Bound: latency, with the special function unit (one exponential a score at 16 per clock) and the
-// issue of the 5.9 instructions that a score takes nearest to full. 32400 tokens, 8 heads of 64: 2.78
+// issue of the 5.9 instructions that a score takes nearest to full. 32400 tokens, 8 heads of 64: 2.77
 // to 3.03 ms (exponentials alone 1.92 ms at 1.85 GHz, products 1.27 ms); counted at 2.94 ms, the unit
 // is 73% busy and issue 0.54. Capped and biased, 128 elements a head: unit 60%, issue 0.42. Tried
 // beside this: issue by lane 0 instead of an elected thread 4.0 ms; two softmax warps per scheduler,
